@@ -1933,8 +1933,8 @@ __device__ __forceinline__ void seg_store_u(uint32_t* p, uint32_t v) { __hip_ato
 __device__ __forceinline__ uint32_t seg_load_u(const uint32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // Record layout: what the walk reads per list entry is a (16 B), the first half of b (8 B) and c (16 B), and the fields sit
-// where the packed fp32 instructions want their operand PAIRS: (x, y) - (px, py), (B2, C2) * dy, (r, g) * w, (b, depth) * w are
-// one v_pk_* each -- same IEEE operations, two per issue slot.
+// next to each other as operand PAIRS: (x, y) - (px, py), (B2, C2) * dy, (r, g) * w, (b, depth) * w.  (The build switches the packed fp32 instructions
+// off: two plain operations each, same bits and, measured, the same rate.)
 typedef float gsr_f32x2 __attribute__((ext_vector_type(2)));
 typedef float gsr_f32x4 __attribute__((ext_vector_type(4)));
 struct SplatLDS {
