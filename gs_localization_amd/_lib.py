@@ -109,6 +109,19 @@ class RefineArgs(C.Structure):
     ]
 
 
+class AdamwArgs(C.Structure):
+    """mirror of `gsr_adamw_args` (include/gsr.h)"""
+    _fields_ = [("n_tensors", _i), ("state_bits", _i), ("tensors", _vp), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("clip", _vp), ("seed", C.c_uint), ("stream", _vp)]
+
+
+class EvictArgs(C.Structure):
+    """mirror of `gsr_evict_args` (include/gsr.h)"""
+    _fields_ = [("P", _i), ("n_views", _i), ("keep", _i), ("recent", _i), ("scores", _vp), ("weights", _vp), ("decay", C.c_double),
+                ("kept", _vp), ("scores_out", _vp), ("n_tensors", _i), ("tensors", _vp), ("workspace", RESIZE_FN), ("workspace_ctx", _vp),
+                ("stream", _vp)]
+
+
 # the GSR_ABI_VERSION these ctypes mirrors (SpecState, RefineArgs, the pose-state layout) were written for
 ABI_VERSION = 5
 REFINE_NO_LEAN, REFINE_SH_SEPARATE, REFINE_NO_BALANCE, REFINE_LOG_REDO, REFINE_DETERMINISTIC, REFINE_NO_SPLIT, REFINE_NO_DILATE = 1, 2, 4, 8, 16, 32, 64
@@ -126,6 +139,12 @@ SIGNATURES.update({
     "gsr_debug_lean_check": (_i, [C.POINTER(RefineArgs), C.POINTER(C.c_longlong)]),
     "gsr_debug_seg_stats": (_i, [C.POINTER(RefineArgs), C.POINTER(C.c_longlong)]),
     "gsr_debug_lam_offset": (C.c_size_t, [_i]),
+    "gsr_grad_norm_bytes": (C.c_size_t, [_i]),
+    "gsr_grad_norm": (_i, [_i, C.POINTER(_vp), C.POINTER(C.c_longlong), C.POINTER(_i), _f, _vp, RESIZE_FN, _vp, _vp]),
+    "gsr_adamw_step": (_i, [C.POINTER(AdamwArgs)]),
+    "gsr_adamw_moments": (_i, [_i, _vp, C.c_double, C.c_double, _i, _vp]),
+    "gsr_evict_bytes": (C.c_size_t, [_i]),
+    "gsr_evict_rows": (_i, [C.POINTER(EvictArgs)]),
     "gsr_grad_mask_bytes": (C.c_size_t, [_i, _i]),
     "gsr_grad_mask": (_i, [_i, _i, _vp, _f, _vp, _i, _i, _vp, _vp, _vp, RESIZE_FN, _vp, _vp]),
     "gsr_grad_mask_replica": (_i, [_i, _i, _vp, _f, _i, _i, _vp, RESIZE_FN, _vp, _vp]),

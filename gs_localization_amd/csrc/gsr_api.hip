@@ -17,6 +17,7 @@
 #include "gsr.h"
 #include "gsr_kernels.h"
 #include "gsr_gradmask.h"
+#include "gsr_mapopt.h"
 
 namespace {
 
@@ -442,6 +443,8 @@ struct ZeroList {
 };
 
 }  // namespace
+
+#include "gsr_mapopt_api.h"          // (with the helpers above)
 
 extern "C" {
 
@@ -2062,6 +2065,34 @@ int gsr_densification_stats(int P, const int* radii, const float* dL_dmean2D, fl
                        max_radii2D, xyz_gradient_accum, denom);
     LAUNCHCHK("k_densification_stats");
     return 0;
+}
+
+// ---- the optimiser step of a map, and its pruning (gsr_mapopt_api.h) ----
+size_t gsr_grad_norm_bytes(int n_tensors) { return (size_t)std::max(1, norm_launches(std::max(0, n_tensors))) * kOptGrid * sizeof(double); }
+
+int gsr_grad_norm(int n_tensors, const void* const* grads, const long long* numels, const int* types, float max_norm, float* out,
+                  gsr_resize_fn workspace, void* workspace_ctx, void* stream)
+{
+    return no_throw([&] { return grad_norm(n_tensors, grads, numels, types, max_norm, out, workspace, workspace_ctx, stream); });
+}
+
+int gsr_adamw_step(const gsr_adamw_args* args)
+{
+    if (!args) return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
+    return no_throw([&] { return adamw_step(args); });
+}
+
+int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream)
+{
+    return no_throw([&] { return adamw_moments(n_tensors, tensors, beta1, beta2, type, stream); });
+}
+
+size_t gsr_evict_bytes(int P) { EvictWs w; return carve_evict(nullptr, P, w); }
+
+int gsr_evict_rows(const gsr_evict_args* args)
+{
+    if (!args) return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
+    return no_throw([&] { return evict_rows(args); });
 }
 
 int gsr_map_from_ply_rows(int P, const float* rows, int row_floats, const int* cols, int n_rest, int activate,

@@ -1,0 +1,277 @@
+// gsr_mapopt_api.h -- host side of gsr_mapopt.h: checks of arguments, tables of a launch, launches.  Part of gsr_api.hip (fail,
+// select_device_of, Carver are its own); the C entry points are there.
+#pragma once
+
+namespace {
+static_assert(sizeof(gsr::OptArgs) <= 4096 && sizeof(gsr::RowArgs) <= 4096 && sizeof(gsr::NormArgs) <= 4096 && sizeof(gsr::MomentArgs) <= 4096,
+              "a launch's table must fit the kernel arguments");
+const long long kOptMaxElements = 1LL << 40;          // (chunks of a launch are counted in 32 bits)
+const int kOptGrid = 2048;                            // workgroups of a launch: eight per CU, each walks chunks
+bool opt_type_ok(int t) { return t == GSR_TYPE_F32 || t == GSR_TYPE_BF16 || t == GSR_TYPE_F16; }
+long long opt_size(int t) { return t == GSR_TYPE_F32 ? 4 : 2; }
+int opt_grid(uint32_t chunks) { return (int)std::max<uint32_t>(1u, std::min<uint32_t>(chunks, (uint32_t)kOptGrid)); }
+
+// Memory that one call writes: no two ranges of it, and no range that it only reads, may overlap.
+struct OptRanges {
+    struct R { uintptr_t lo, hi; bool write; };
+    std::vector<R> r;
+    void add(const void* p, long long bytes, bool write) { if (p && bytes > 0) r.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, write}); }
+    bool clash()
+    {
+        std::sort(r.begin(), r.end(), [](const R& a, const R& b) { return a.lo < b.lo; });
+        uintptr_t end = 0, wend = 0;          // of everything so far, and of what is written
+        for (const R& x : r) {
+            if (x.lo < wend || (x.write && x.lo < end)) return true;
+            end = std::max(end, x.hi);
+            if (x.write) wend = std::max(wend, x.hi);
+        }
+        return false;
+    }
+};
+
+int adamw_step(const gsr_adamw_args* a)
+{
+    using namespace gsr;
+    const int debug = 0;
+    hipStream_t st = (hipStream_t)a->stream;
+    if (a->n_tensors < 0 || (a->n_tensors > 0 && !a->tensors)) return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
+    if (a->state_bits != 32 && a->state_bits != 8) return fail(GSR_E_INVALID, "gsr_adamw_step: moments have 32 or 8 bits%s", "");
+    if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: 0 <= beta < 1 required%s", "");
+    if (!(a->eps >= 0.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: eps >= 0 required%s", "");
+    const bool eight = a->state_bits == 8;
+    if (eight && !(a->beta1 * a->beta1 < a->beta2)) return fail(GSR_E_INVALID, "gsr_adamw_step: 8-bit moments need beta1^2 < beta2 (otherwise m / sqrt(v) has no bound)%s", "");
+    if (a->n_tensors == 0) return 0;
+    OptRanges ranges;
+    ranges.r.reserve((size_t)a->n_tensors * 6 + 1);
+    for (int i = 0; i < a->n_tensors; i++) {
+        const gsr_opt_tensor& t = a->tensors[i];
+        if (t.n < 0 || t.n > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_adamw_step: bad tensor size%s", "");
+        if (!opt_type_ok(t.param_type) || !opt_type_ok(t.grad_type)) return fail(GSR_E_INVALID, "gsr_adamw_step: unknown type%s", "");
+        if (!t.clock || (t.n > 0 && (!t.param || !t.grad || !t.state0 || !t.state1 || (eight && !t.window))))
+            return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
+        if (((uintptr_t)t.clock & 7) || (((uintptr_t)t.param) & (uintptr_t)(opt_size(t.param_type) - 1)) || (((uintptr_t)t.grad) & (uintptr_t)(opt_size(t.grad_type) - 1)) ||
+            (!eight && (((uintptr_t)t.state0 | (uintptr_t)t.state1) & 3)))
+            return fail(GSR_E_INVALID, "gsr_adamw_step: a pointer is not aligned to its type%s", "");
+        ranges.add(t.param, t.n * opt_size(t.param_type), true);
+        ranges.add(t.state0, t.n * (eight ? 1 : 4), true);
+        ranges.add(t.state1, t.n * (eight ? 1 : 4), true);
+        if (eight) ranges.add(t.window, (t.n + GSR_OPT_WINDOW - 1) / GSR_OPT_WINDOW, true);
+        ranges.add(t.clock, 4 * sizeof(double), true);
+        ranges.add(t.grad, t.n * opt_size(t.grad_type), false);
+        ranges.add(t.lr_device, sizeof(double), false);
+    }
+    ranges.add(a->clip, 2 * sizeof(float), false);
+    if (ranges.clash()) return fail(GSR_E_INVALID, "gsr_adamw_step: memory that the step writes overlaps other memory of the call (a tensor given twice?)%s", "");
+    int rc = select_device_of(a->tensors[0].clock);
+    if (rc != GSR_OK) return rc;
+    OptArgs k;
+    k.beta1 = a->beta1; k.beta2 = a->beta2;
+    k.b1 = (float)a->beta1; k.b2 = (float)a->beta2; k.c1 = (float)(1.0 - a->beta1); k.c2 = (float)(1.0 - a->beta2); k.eps = (float)a->eps;
+    k.clip = a->clip;
+    const double span = eight ? (1.0 - a->beta1) / sqrt((1.0 - a->beta2) * (1.0 - a->beta1 * a->beta1 / a->beta2)) : 1.0;
+    k.unit = (float)(span / 127.0); k.per_unit = (float)(127.0 / span);
+    k.count = 0; k.chunks = 0;
+    for (int i = 0; i < a->n_tensors; i++) {
+        const gsr_opt_tensor& t = a->tensors[i];
+        const uint32_t chunks = (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+        OptTensor& o = k.t[k.count++];
+        o.p = t.param; o.g = t.grad; o.s0 = t.state0; o.s1 = t.state1; o.window = t.window; o.clock = t.clock; o.lr_device = t.lr_device;
+        o.lr = t.lr; o.decay = t.weight_decay; o.n = t.n; o.first = k.chunks;
+        o.key = a->seed * 0x9E3779B1u + (uint32_t)(i + 1) * 0x85EBCA77u;
+        o.types = t.param_type | t.grad_type << 4;
+        k.chunks += chunks;
+        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
+        if (!full && i + 1 < a->n_tensors) continue;
+        if (eight) {
+            hipLaunchKernelGGL(k_adamw8, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+            LAUNCHCHK("k_adamw8");
+        } else {
+            hipLaunchKernelGGL(k_adamw, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+            LAUNCHCHK("k_adamw");
+        }
+        k.count = 0; k.chunks = 0;
+    }
+    return 0;
+}
+
+int adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream)
+{
+    using namespace gsr;
+    const int debug = 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return fail(GSR_E_INVALID, "gsr_adamw_moments: NULL pointer%s", "");
+    if (!opt_type_ok(type)) return fail(GSR_E_INVALID, "gsr_adamw_moments: unknown type%s", "");
+    if (!(beta1 >= 0.0 && beta2 < 1.0 && beta1 * beta1 < beta2)) return fail(GSR_E_INVALID, "gsr_adamw_moments: 0 <= beta1, beta1^2 < beta2 < 1 required%s", "");
+    OptRanges ranges;
+    const void* any = nullptr;
+    for (int i = 0; i < n_tensors; i++) {
+        const gsr_moment_tensor& t = tensors[i];
+        if (t.n < 0 || t.n > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_adamw_moments: bad tensor size%s", "");
+        if (t.n > 0 && (!t.rms || !t.ratio || !t.window || !t.exp_avg_out || !t.rms_out)) return fail(GSR_E_INVALID, "gsr_adamw_moments: NULL pointer%s", "");
+        if (((uintptr_t)t.exp_avg_out | (uintptr_t)t.rms_out) & (uintptr_t)(opt_size(type) - 1)) return fail(GSR_E_INVALID, "gsr_adamw_moments: a pointer is not aligned to its type%s", "");
+        ranges.add(t.rms, t.n, false); ranges.add(t.ratio, t.n, false); ranges.add(t.window, (t.n + GSR_OPT_WINDOW - 1) / GSR_OPT_WINDOW, false);
+        ranges.add(t.exp_avg_out, t.n * opt_size(type), true); ranges.add(t.rms_out, t.n * opt_size(type), true);
+        if (t.n > 0) any = t.rms;
+    }
+    if (!any) return 0;
+    if (ranges.clash()) return fail(GSR_E_INVALID, "gsr_adamw_moments: an output overlaps other memory of the call%s", "");
+    int rc = select_device_of(any);
+    if (rc != GSR_OK) return rc;
+    MomentArgs k;
+    k.unit = (float)((1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)) / 127.0);
+    k.type = type; k.count = 0; k.chunks = 0;
+    for (int i = 0; i < n_tensors; i++) {
+        const gsr_moment_tensor& t = tensors[i];
+        if (t.n > 0) {
+            MomentTensor& o = k.t[k.count++];
+            o.rms = t.rms; o.ratio = t.ratio; o.window = t.window; o.exp_avg = t.exp_avg_out; o.root = t.rms_out; o.n = t.n; o.first = k.chunks;
+            k.chunks += (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+        }
+        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
+        if (k.count == 0 || (!full && i + 1 < n_tensors)) continue;
+        hipLaunchKernelGGL(k_moments8, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+        LAUNCHCHK("k_moments8");
+        k.count = 0; k.chunks = 0;
+    }
+    return 0;
+}
+
+int norm_launches(int n_tensors) { return (n_tensors + GSR_NORM_MAX - 1) / GSR_NORM_MAX; }
+
+int grad_norm(int n_tensors, const void* const* grads, const long long* numels, const int* types, float max_norm, float* out,
+              gsr_resize_fn workspace, void* workspace_ctx, void* stream)
+{
+    using namespace gsr;
+    const int debug = 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (n_tensors < 0 || (n_tensors > 0 && (!grads || !numels || !types)) || !out || !workspace) return fail(GSR_E_INVALID, "gsr_grad_norm: NULL pointer%s", "");
+    if (!(max_norm >= 0.0f)) return fail(GSR_E_INVALID, "gsr_grad_norm: max_norm >= 0 required%s", "");
+    for (int i = 0; i < n_tensors; i++) {
+        if (numels[i] < 0 || numels[i] > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_grad_norm: bad tensor size%s", "");
+        if (!opt_type_ok(types[i])) return fail(GSR_E_INVALID, "gsr_grad_norm: unknown type%s", "");
+        if (numels[i] > 0 && (!grads[i] || ((uintptr_t)grads[i] & (uintptr_t)(opt_size(types[i]) - 1)))) return fail(GSR_E_INVALID, "gsr_grad_norm: NULL or unaligned gradient%s", "");
+    }
+    int rc = select_device_of(out);
+    if (rc != GSR_OK) return rc;
+    double* partial = (double*)workspace(workspace_ctx, gsr_grad_norm_bytes(n_tensors));
+    if (!partial) return fail(GSR_E_ALLOC, "workspace callback returned NULL%s", "");
+    NormArgs k;
+    k.count = 0; k.chunks = 0;
+    int sums = 0;
+    for (int i = 0; i < n_tensors; i++) {
+        if (numels[i] > 0) {
+            k.t[k.count++] = {grads[i], numels[i], k.chunks, types[i]};
+            k.chunks += (uint32_t)((numels[i] + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+        }
+        const bool full = k.count == GSR_NORM_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
+        if (k.count == 0 || (!full && i + 1 < n_tensors)) continue;
+        k.partial = partial + sums;
+        const int grid = opt_grid(k.chunks);
+        hipLaunchKernelGGL(k_grad_norm, dim3(grid), dim3(GSR_OPT_THREADS), 0, st, k);
+        LAUNCHCHK("k_grad_norm");
+        sums += grid;
+        k.count = 0; k.chunks = 0;
+    }
+    hipLaunchKernelGGL(k_grad_norm_finish, dim3(1), dim3(GSR_OPT_THREADS), 0, st, (const double*)partial, sums, max_norm, out);
+    LAUNCHCHK("k_grad_norm_finish");
+    return 0;
+}
+
+struct EvictWs { uint32_t* hist; uint2* counts; float* total; };
+size_t carve_evict(char* base, int P, EvictWs& w)
+{
+    Carver c(base);
+    w.hist = c.take<uint32_t>(3 * GSR_EV_BINS);
+    w.counts = c.take<uint2>(GSR_EV_TILES);
+    w.total = c.take<float>(P > 0 ? (size_t)P : 1);
+    return c.size();
+}
+
+int evict_rows(const gsr_evict_args* a)
+{
+    using namespace gsr;
+    const int debug = 0;
+    hipStream_t st = (hipStream_t)a->stream;
+    if (a->P < 0 || a->n_views < 0 || a->n_tensors < 0) return fail(GSR_E_INVALID, "gsr_evict_rows: negative size%s", "");
+    if (!(a->recent >= 0 && a->recent <= a->keep && a->keep <= a->P)) return fail(GSR_E_INVALID, "gsr_evict_rows: 0 <= recent <= keep <= P required%s", "");
+    if (a->n_tensors > 0 && !a->tensors) return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
+    for (int i = 0; i < a->n_tensors; i++) {
+        const gsr_row_tensor& t = a->tensors[i];
+        if (t.row_bytes < 0 || t.row_bytes * (long long)a->P > 4 * kOptMaxElements || t.row_bytes > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_evict_rows: bad row size%s", "");
+        if (a->keep > 0 && t.row_bytes > 0 && (!t.src || !t.dst || (t.src_window != nullptr) != (t.dst_window != nullptr)))
+            return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
+    }
+    if (a->keep == 0) return 0;
+    if (!a->scores || !a->kept || !a->scores_out || !a->workspace || (a->n_views > 0 && !a->weights)) return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
+    OptRanges ranges;
+    ranges.add(a->scores, 4LL * a->P, false); ranges.add(a->weights, 4LL * a->P * a->n_views, false);
+    ranges.add(a->kept, 8LL * a->keep, true); ranges.add(a->scores_out, 4LL * a->keep, true);
+    for (int i = 0; i < a->n_tensors; i++) {
+        const gsr_row_tensor& t = a->tensors[i];
+        ranges.add(t.src, t.row_bytes * a->P, false); ranges.add(t.dst, t.row_bytes * a->keep, true);
+        if (t.src_window) {
+            ranges.add(t.src_window, (t.row_bytes * a->P + GSR_OPT_WINDOW - 1) / GSR_OPT_WINDOW, false);
+            ranges.add(t.dst_window, (t.row_bytes * a->keep + GSR_OPT_WINDOW - 1) / GSR_OPT_WINDOW, true);
+        }
+    }
+    if (ranges.clash()) return fail(GSR_E_INVALID, "gsr_evict_rows: an output overlaps other memory of the call%s", "");
+    int rc = select_device_of(a->scores);
+    if (rc != GSR_OK) return rc;
+    EvictWs w;
+    char* ws = (char*)a->workspace(a->workspace_ctx, carve_evict(nullptr, a->P, w));
+    if (!ws) return fail(GSR_E_ALLOC, "workspace callback returned NULL%s", "");
+    carve_evict(ws, a->P, w);
+    EvictArgs e;
+    e.P = a->P; e.views = a->n_views; e.old = a->P - a->recent; e.k = a->keep - a->recent; e.decay = a->decay;
+    e.scores = a->scores; e.weights = a->weights; e.total = w.total; e.hist = w.hist; e.counts = w.counts;
+    e.kept = a->kept; e.scores_out = a->scores_out;
+    const int per = (int)(((long long)a->P + GSR_EV_TILES - 1) / GSR_EV_TILES);
+    e.tile_rows = (int)std::max<long long>(1024, ((long long)per + 255) / 256 * 256);
+    e.tiles = (int)(((long long)a->P + e.tile_rows - 1) / e.tile_rows);
+    ClearRanges cr = {};
+    cr.p[0] = w.hist; cr.n[0] = 3 * GSR_EV_BINS;
+    hipLaunchKernelGGL(k_refine_init, dim3(3 * GSR_EV_BINS / GSR_BLOCK), dim3(GSR_BLOCK), 0, st, cr, PoseLoadArgs{});
+    LAUNCHCHK("k_refine_init");
+    const int blocks = (int)std::min<long long>(((long long)a->P + 255) / 256, 1024);
+    hipLaunchKernelGGL(k_evict_scores, dim3(blocks), dim3(256), 0, st, e);
+    LAUNCHCHK("k_evict_scores");
+    if (e.k > 0 && e.k < e.old) {
+        hipLaunchKernelGGL(k_evict_hist<2>, dim3(blocks), dim3(256), 0, st, e);
+        LAUNCHCHK("k_evict_hist<2>");
+        hipLaunchKernelGGL(k_evict_hist<3>, dim3(blocks), dim3(256), 0, st, e);
+        LAUNCHCHK("k_evict_hist<3>");
+    }
+    hipLaunchKernelGGL(k_evict_count, dim3(e.tiles), dim3(256), 0, st, e);
+    LAUNCHCHK("k_evict_count");
+    hipLaunchKernelGGL(k_evict_emit, dim3(e.tiles), dim3(256), 0, st, e);
+    LAUNCHCHK("k_evict_emit");
+    RowArgs k;
+    k.keep = a->keep; k.kept = a->kept; k.count = 0; k.chunks = 0;
+    for (int i = 0; i < a->n_tensors; i++) {
+        const gsr_row_tensor& t = a->tensors[i];
+        if (t.row_bytes > 0) {
+            RowTensor& o = k.t[k.count++];
+            o.src = t.src; o.dst = t.dst; o.src_window = t.src_window; o.dst_window = t.dst_window; o.first = k.chunks; o.pad = 0;
+            const uintptr_t bits = (uintptr_t)t.src | (uintptr_t)t.dst | (uintptr_t)t.row_bytes;
+            o.unit = t.src_window ? 1 : (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
+            o.row = t.row_bytes / o.unit;
+            k.chunks += (uint32_t)((o.row * a->keep + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+        }
+        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x40000000u;
+        if (k.count == 0 || (!full && i + 1 < a->n_tensors)) continue;
+        hipLaunchKernelGGL(k_evict_rows, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+        LAUNCHCHK("k_evict_rows");
+        k.count = 0; k.chunks = 0;
+    }
+    return 0;
+}
+
+// std::vector and std::sort may throw; nothing may leave a C entry point that way.
+template <class F>
+int no_throw(F f)
+{
+    try { return f(); }
+    catch (const std::exception& e) { return fail(GSR_E_ALLOC, "host memory: %s", e.what()); }
+    catch (...) { return fail(GSR_E_ALLOC, "host exception%s", ""); }
+}
+}  // namespace

@@ -1,0 +1,414 @@
+"""The optimiser step of a Gaussian map and the pruning that goes with it, on hand-written HIP kernels (include/gsr.h: gsr_grad_norm,
+gsr_adamw_step, gsr_adamw_moments, gsr_evict_rows).
+
+gaussian_splatting/train.py:156-158 steps torch.optim.Adam over the six tensors of a map and gaussian_splatting/scene/
+gaussian_model.py:269-328 rewrites its state whenever splats are pruned or added.  Here
+
+  AdamW           an optimiser with torch's constructor, groups and state ("exp_avg", "exp_avg_sq"): one launch for all tensors; moments
+                  in 32 bits or in a byte each (state_bits=8: 16 instead of 28 bytes of traffic per fp32 parameter, 2 instead
+                  of 8 bytes of state); clipping by the gradients' norm without a read-back; evict() and append_rows() for its maps
+  grad_norm, adamw_step, adamw_step_8bit, moments_8bit, evict_rows      the operators by themselves
+  compositing_weights                                                   what evict_rows accumulates, from the rasterizer
+
+No entry point reads anything back, and each runs on its tensors' device and that device's current stream.  Nothing falls back to torch
+or to the CPU: tensors elsewhere are refused.  Tensors that a step writes must be contiguous and must not overlap (refused); the
+step counts live on the device, so a captured graph counts on when it is replayed."""
+import ctypes as C
+import math
+import struct
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_OPT = struct.Struct("7Q2dq2i")          # gsr_opt_tensor
+_MOMENT = struct.Struct("5Qq")           # gsr_moment_tensor
+_ROW = struct.Struct("4Qq")              # gsr_row_tensor
+WINDOW = 256                             # elements that share a window byte of the 8-bit root
+
+
+def _device(tensors, name):
+    """The one HIP device that all of them live on."""
+    dev = None
+    for t in tensors:
+        if not torch.is_tensor(t):
+            raise TypeError(f"{name} needs tensors, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} needs HIP tensors (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"{name}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _type(t, name):
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"{name}: {t.dtype} is not supported (float32, bfloat16, float16)") from None
+
+
+class _on:
+    """The device as the current one (the stream is its current stream)."""
+
+    def __init__(self, dev):
+        self.index = dev.index
+        self.back = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.index != self.back:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        torch.cuda.set_device(self.back)          # (the library selects a device by itself)
+
+
+def _workspace(nbytes, dev):
+    t = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return t, _lib.FixedBuffer(t.data_ptr(), nbytes, 0)
+
+
+def _address(buf):
+    return C.addressof(C.c_char.from_buffer(buf)) if buf else None
+
+
+def grad_norm(grads, max_norm=math.inf):
+    """grads: tensors (float32, bfloat16, float16; any sizes).  Returns a float32 tensor (norm, coefficient) on their device: the 2-norm over
+    all of them (64-bit sums in a fixed order) and min(1, max_norm / (norm + 1e-6)), what torch.nn.utils.clip_grad_norm_ would multiply them
+    by -- handed to adamw_step as `clip` no gradient is written.  A NaN or infinite gradient gives a norm that says so."""
+    lib = _lib.load()
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not grads:
+        raise ValueError("grad_norm: no gradients")
+    if not max_norm >= 0.0:
+        raise ValueError(f"grad_norm: max_norm >= 0 required, got {max_norm}")
+    dev = _device(grads, "grad_norm")
+    n = len(grads)
+    types = (C.c_int * n)(*[_type(g, "grad_norm") for g in grads])
+    ptrs = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    numels = (C.c_longlong * n)(*[g.numel() for g in grads])
+    with _on(dev) as stream:
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        keep, ws = _workspace(lib.gsr_grad_norm_bytes(n), dev)
+        _lib.check(lib.gsr_grad_norm(n, ptrs, numels, types, max_norm, out.data_ptr(), _lib.fixed_buffer_fn(), C.addressof(ws), stream))
+    return out
+
+
+def _per_tensor(x, n, name):
+    if isinstance(x, (list, tuple)):
+        if len(x) != n:
+            raise ValueError(f"{name}: {len(x)} values for {n} tensors")
+        return x
+    return [x] * n
+
+
+def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed):
+    lib = _lib.load()
+    n = len(params)
+    if not (len(grads) == len(state0) == len(state1) == len(clocks) == n) or (windows is not None and len(windows) != n):
+        raise ValueError(f"{name}: lists of different lengths")
+    if n == 0:
+        return
+    lrs, decays = _per_tensor(lr, n, name + ": lr"), _per_tensor(weight_decay, n, name + ": weight_decay")
+    d0, d1 = (torch.float32, torch.float32) if bits == 32 else (torch.uint8, torch.int8)
+    dev = params[0].device
+    if clip is not None and not (clip.dtype is torch.float32 and clip.numel() == 2 and clip.is_contiguous() and clip.device == dev):
+        raise ValueError(f"{name}: clip is grad_norm's result (two float32 on the parameters' device)")
+    buf, keep, written = bytearray(_OPT.size * n), [], []
+    for i in range(n):
+        p, g, a, b, clock, rate = params[i], grads[i], state0[i], state1[i], clocks[i], lrs[i]
+        w = windows[i] if windows is not None else None
+        k = p.numel()
+        _device((p, g, a, b, clock) if w is None else (p, g, a, b, clock, w), name)
+        if p.device != dev:
+            raise RuntimeError(f"{name}: tensors on {dev} and {p.device}")
+        if a.dtype is not d0 or b.dtype is not d1 or clock.dtype is not torch.float64 or (w is not None and w.dtype is not torch.uint8):
+            raise TypeError(f"{name}: tensor {i}: moments are {d0} and {d1}, the clock float64" + (", the window uint8" if bits == 8 else ""))
+        if g.shape != p.shape or a.numel() != k or b.numel() != k or clock.numel() != 4 or (w is not None and w.numel() != (k + WINDOW - 1) // WINDOW):
+            raise ValueError(f"{name}: tensor {i}: sizes do not match the parameter's {tuple(p.shape)}")
+        if not (p.is_contiguous() and a.is_contiguous() and b.is_contiguous() and clock.is_contiguous() and (w is None or w.is_contiguous())):
+            raise ValueError(f"{name}: tensor {i}: what the step writes must be contiguous")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        lr_ptr = 0
+        if torch.is_tensor(rate):
+            if not (rate.dtype is torch.float64 and rate.numel() == 1 and rate.device == dev):
+                raise ValueError(f"{name}: lr as a tensor is one float64 on the parameters' device")
+            lr_ptr, rate = rate.data_ptr(), 0.0
+        _OPT.pack_into(buf, _OPT.size * i, p.data_ptr(), g.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if w is None else w.data_ptr(),
+                       clock.data_ptr(), lr_ptr, rate, decays[i], k, _type(p, name), _type(g, name))
+        written += (p, a, b, clock) if w is None else (p, a, b, clock, w)
+    with _on(dev) as stream:
+        args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, stream)
+        _lib.check(lib.gsr_adamw_step(C.byref(args)))
+    torch.autograd.graph.increment_version(written)
+
+
+def new_clock(device):
+    """The step count of one tensor: beta1^t, beta2^t, t and a word of the kernel's own, in 64 bits on the device."""
+    return torch.tensor([1.0, 1.0, 0.0, 0.0], dtype=torch.float64, device=device)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, clocks, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, clip=None):
+    """One AdamW step over many tensors in one launch, in place (torch.optim.AdamW; with weight_decay 0 torch.optim.Adam).
+    params, grads: float32, bfloat16 or float16; exp_avgs, exp_avg_sqs: float32, zero before the first step; clocks: new_clock() each.
+    lr, weight_decay: one number or one per tensor; an lr may be a float64 tensor of one element on the device, which a replayed graph
+    reads anew.  clip: what grad_norm returned, or None.  A gradient that is not contiguous is copied."""
+    _step(32, "adamw_step", params, grads, exp_avgs, exp_avg_sqs, None, clocks, lr, betas, eps, weight_decay, clip, 0)
+
+
+def adamw_step_8bit(params, grads, rms, ratio, window, clocks, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, clip=None, seed=0):
+    """adamw_step with a byte for each moment: rms (uint8, sqrt(exp_avg_sq) to a sixteenth of its binade), ratio (int8, exp_avg / sqrt(exp_avg_sq)
+    in 127 steps of the largest it can be), window (uint8, one per 256 elements of the flattened tensor: which sixteen binades rms
+    covers); all zero before the first step.  Rounding is stochastic, from `seed`, the step and the element's place: the same
+    call on the same state gives the same bits.  Needs beta1^2 < beta2.  moments_8bit reads them."""
+    _step(8, "adamw_step_8bit", params, grads, rms, ratio, window, clocks, lr, betas, eps, weight_decay, clip, seed)
+
+
+def moments_8bit(rms, ratio, window, betas=(0.9, 0.999), dtype=torch.float32):
+    """The moments that adamw_step_8bit's bytes stand for, as two lists of tensors: exp_avg and sqrt(exp_avg_sq)."""
+    lib = _lib.load()
+    n = len(rms)
+    if len(ratio) != n or len(window) != n:
+        raise ValueError("moments_8bit: lists of different lengths")
+    if dtype not in _TYPES:
+        raise TypeError(f"moments_8bit: {dtype} is not supported (float32, bfloat16, float16)")
+    if n == 0:
+        return [], []
+    dev = _device([*rms, *ratio, *window], "moments_8bit")
+    buf, avg, root = bytearray(_MOMENT.size * n), [], []
+    with _on(dev) as stream:
+        for i, (c, r, w) in enumerate(zip(rms, ratio, window)):
+            k = c.numel()
+            if c.dtype is not torch.uint8 or r.dtype is not torch.int8 or w.dtype is not torch.uint8 or r.numel() != k or w.numel() != (k + WINDOW - 1) // WINDOW:
+                raise ValueError(f"moments_8bit: tensor {i}: rms uint8 [n], ratio int8 [n], window uint8 [(n + {WINDOW - 1}) // {WINDOW}] required")
+            if not (c.is_contiguous() and r.is_contiguous() and w.is_contiguous()):
+                raise ValueError(f"moments_8bit: tensor {i} is not contiguous")
+            avg.append(torch.empty(c.shape, dtype=dtype, device=dev))
+            root.append(torch.empty(c.shape, dtype=dtype, device=dev))
+            _MOMENT.pack_into(buf, _MOMENT.size * i, c.data_ptr(), r.data_ptr(), w.data_ptr(), avg[i].data_ptr(), root[i].data_ptr(), k)
+        _lib.check(lib.gsr_adamw_moments(n, _address(buf), betas[0], betas[1], _TYPES[dtype], stream))
+    return avg, root
+
+
+def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=()):
+    """Compacts a map to `keep` of its P rows by accumulated compositing weight.
+
+    scores: float32 [P], accumulated so far; weights: float32 [views, P] or [P], this round's (compositing_weights), or None:
+    score = decay * score + sum of weights.  The last `recent` rows stay whatever their score, and of the others the keep - recent with
+    the largest (ties: the lower index; NaN counts as -inf).  tensors: [P, ...] each, of any types; rms: pairs (codes uint8 [P, ...], window)
+    of 8-bit moments, re-coded for their new blocks -- exact, but for a root under its new window's sixteen binades, which
+    becomes that window's lowest value.
+    Returns (kept int64 [keep] ascending, scores [keep], [tensor [keep, ...]], [(codes, window)]); the inputs are not written."""
+    lib = _lib.load()
+    P, keep, recent = scores.numel(), int(keep), int(recent)
+    if scores.dim() != 1 or scores.dtype is not torch.float32:
+        raise ValueError("evict_rows: scores is float32 [P]")
+    if not 0 <= recent <= keep <= P:
+        raise ValueError(f"evict_rows: 0 <= recent <= keep <= P required, got recent {recent}, keep {keep}, P {P}")
+    if P > 0x7FFFFFFF:
+        raise ValueError("evict_rows: at most 2^31 - 1 rows")
+    if weights is not None:
+        weights = (weights if weights.dim() == 2 else weights.unsqueeze(0)).contiguous()
+        if weights.dtype is not torch.float32 or weights.dim() != 2 or weights.shape[1] != P:
+            raise ValueError("evict_rows: weights is float32 [views, P] or [P]")
+    scores = scores.contiguous()
+    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    rms = [(c if c.is_contiguous() else c.contiguous(), w if w.is_contiguous() else w.contiguous()) for c, w in rms]
+    dev = _device([scores] + ([] if weights is None else [weights]) + tensors + [x for pair in rms for x in pair], "evict_rows")
+    n = len(tensors) + len(rms)
+    buf, rows, pairs = bytearray(_ROW.size * n), [], []
+    with _on(dev) as stream:
+        kept = torch.empty(keep, dtype=torch.int64, device=dev)
+        out = torch.empty(keep, dtype=torch.float32, device=dev)
+        for i, t in enumerate(tensors):
+            if t.dim() < 1 or t.shape[0] != P:
+                raise ValueError(f"evict_rows: tensor {i} has shape {tuple(t.shape)}, {P} rows wanted")
+            rows.append(torch.empty((keep, *t.shape[1:]), dtype=t.dtype, device=dev))
+            _ROW.pack_into(buf, _ROW.size * i, t.data_ptr(), rows[i].data_ptr(), 0, 0, t.element_size() * (t.numel() // P) if P else 0)
+        for i, (c, w) in enumerate(rms):
+            if c.dim() < 1 or c.shape[0] != P or c.dtype is not torch.uint8 or w.dtype is not torch.uint8 or w.numel() != (c.numel() + WINDOW - 1) // WINDOW:
+                raise ValueError(f"evict_rows: rms {i}: codes uint8 [P, ...] and their window uint8 required")
+            row = c.numel() // P if P else 0
+            pairs.append((torch.empty((keep, *c.shape[1:]), dtype=torch.uint8, device=dev),
+                          torch.empty((keep * row + WINDOW - 1) // WINDOW, dtype=torch.uint8, device=dev)))
+            _ROW.pack_into(buf, _ROW.size * (len(tensors) + i), c.data_ptr(), pairs[i][0].data_ptr(), w.data_ptr(), pairs[i][1].data_ptr(), row)
+        ws_t, ws = _workspace(lib.gsr_evict_bytes(P), dev)
+        args = _lib.EvictArgs(P, 0 if weights is None else weights.shape[0], keep, recent, scores.data_ptr(),
+                              None if weights is None else weights.data_ptr(), decay, kept.data_ptr(), out.data_ptr(), n, _address(buf),
+                              _lib.fixed_buffer_fn(), C.addressof(ws), stream)
+        _lib.check(lib.gsr_evict_rows(C.byref(args)))
+    return kept, out, rows, pairs
+
+
+def compositing_weights(raster_settings, means3D, opacities, scales=None, rotations=None, cov3D_precomp=None):
+    """float32 [P]: how much each splat contributes to the view that raster_settings (diff_gaussian_rasterization's) describes, the sum over
+    pixels of alpha_i T_i -- the derivative of a colour channel's sum by the splat's own colour, so one forward and backward of the
+    rasterizer.  What evict_rows accumulates over views."""
+    from .rasterizer import GaussianRasterizer
+    det = lambda t: None if t is None else t.detach()                                             # noqa: E731
+    with torch.enable_grad():
+        colors = torch.zeros(means3D.shape[0], 3, dtype=torch.float32, device=means3D.device, requires_grad=True)
+        image = GaussianRasterizer(raster_settings)(means3D=det(means3D), means2D=torch.zeros_like(det(means3D)), opacities=det(opacities),
+                                                    colors_precomp=colors, scales=det(scales), rotations=det(rotations),
+                                                    cov3D_precomp=det(cov3D_precomp))[0]
+        ones = torch.zeros_like(image)
+        ones[0] = 1.0
+        return torch.autograd.grad(image, colors, ones)[0][:, 0].contiguous()
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.Adam / AdamW for the tensors of a map: `AdamW(groups, lr=0.0, eps=1e-15)` where train.py's
+    training_setup (gaussian_splatting/scene/gaussian_model.py:149-167) has `torch.optim.Adam(groups, lr=0.0, eps=1e-15)`.
+
+    weight_decay is decoupled (0, Adam, by default).  state_bits=8 (per group) keeps the moments in two bytes per element; seed is
+    that of their stochastic rounding.  max_norm clips every step by the norm over all groups' gradients, last_norm is then that step's
+    (norm, coefficient) on the device.  With 32 bits the state holds "exp_avg" and "exp_avg_sq", shaped like the parameter,
+    so code that indexes, concatenates or replaces them goes on working; with 8 bits "rms" and "ratio" are shaped like the parameter and
+    "window" is one byte per 256 elements -- use evict() and append_rows(), which know all of them.  "step" is new_clock()."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=32, max_norm=None, seed=0):
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError(f"max_norm >= 0 required, got {max_norm}")
+        self.max_norm, self.seed, self.last_norm = max_norm, int(seed), None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        b1, b2 = g["betas"]
+        try:
+            if not (torch.is_tensor(g["lr"]) or g["lr"] >= 0.0):
+                raise ValueError(f"lr >= 0 required, got {g['lr']}")
+            if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+                raise ValueError(f"0 <= beta < 1 required, got {g['betas']}")
+            if not g["eps"] >= 0.0 or not g["weight_decay"] >= 0.0:
+                raise ValueError(f"eps >= 0 and weight_decay >= 0 required, got {g['eps']}, {g['weight_decay']}")
+            if g["state_bits"] not in (32, 8):
+                raise ValueError(f"state_bits is 32 or 8, got {g['state_bits']}")
+            if g["state_bits"] == 8 and not b1 * b1 < b2:
+                raise ValueError(f"8-bit moments need beta1^2 < beta2 (otherwise exp_avg / sqrt(exp_avg_sq) has no bound), got {g['betas']}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def _init_state(self, p, bits):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a parameter's first step cannot be captured (its state would start anew at every replay): step once before")
+        st = self.state[p]
+        like = lambda dt: torch.zeros(p.shape, dtype=dt, device=p.device)                          # noqa: E731
+        if bits == 32:
+            st["exp_avg"], st["exp_avg_sq"] = like(torch.float32), like(torch.float32)
+        else:
+            st["rms"], st["ratio"] = like(torch.uint8), like(torch.int8)
+            st["window"] = torch.zeros((p.numel() + WINDOW - 1) // WINDOW, dtype=torch.uint8, device=p.device)
+        st["step"] = new_clock(p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls, grads = {}, []
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.layout is not torch.strided:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                _device((p,), "AdamW")
+                st = self.state[p] if p in self.state else None
+                if not st:
+                    st = self._init_state(p, group["state_bits"])
+                call = calls.setdefault((group["state_bits"], tuple(group["betas"]), group["eps"]), ([], [], [], [], [], [], [], []))
+                for x, y in zip(call, (p, p.grad, *((st["exp_avg"], st["exp_avg_sq"], None) if group["state_bits"] == 32 else
+                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"])):
+                    x.append(y)
+                grads.append(p.grad)
+        if not grads:
+            return loss
+        clip = None
+        if self.max_norm is not None:
+            clip = self.last_norm = grad_norm(grads, self.max_norm)
+        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd) in calls.items():
+            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """Takes its own state_dict() and torch.optim.Adam's / AdamW's (32-bit groups): states keep their types whatever the parameter's."""
+        own, given = self.param_groups, state_dict["param_groups"]
+        bits = [g.get("state_bits", own[k]["state_bits"]) if k < len(own) else 32 for k, g in enumerate(given)]
+        for b, g in zip(bits, given):
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("load_state_dict: amsgrad and maximize are not supported")
+            wanted = {"exp_avg", "exp_avg_sq", "step"} if b == 32 else {"rms", "ratio", "window", "step"}
+            for i in g["params"]:
+                if i in state_dict["state"] and not wanted <= set(state_dict["state"][i]):
+                    raise ValueError(f"load_state_dict: a group with {b}-bit moments got the state {sorted(state_dict['state'][i])}")
+        super().load_state_dict(state_dict)
+        for b, g, old in zip(bits, self.param_groups, given):
+            for k in set(g) - {"params", "name", "state_bits", *self.defaults} - set(own[0]):
+                del g[k]          # (torch's own options: capturable, foreach, ...)
+            g["state_bits"] = b
+            for i, p in zip(old["params"], g["params"]):
+                if i not in state_dict["state"]:
+                    continue
+                # (the base class casts every state to the parameter's type)
+                st = {k: v.detach().to(device=p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][i].items()}
+                if not torch.is_tensor(st["step"]) or st["step"].numel() == 1:
+                    t = float(st["step"])
+                    st["step"] = torch.tensor([g["betas"][0] ** t, g["betas"][1] ** t, t, 0.0], dtype=torch.float64, device=p.device)
+                if b == 32:
+                    st["exp_avg"], st["exp_avg_sq"] = st["exp_avg"].float(), st["exp_avg_sq"].float()
+                self.state[p] = st
+
+    def _replace(self, old, data, states):
+        new = torch.nn.Parameter(data, requires_grad=old.requires_grad)
+        st = self.state.pop(old, None)
+        if st:
+            self.state[new] = dict(st, **states)
+        for g in self.param_groups:
+            g["params"] = [new if p is old else p for p in g["params"]]
+
+    @torch.no_grad()
+    def evict(self, scores, keep, recent=0, weights=None, decay=1.0, extra=()):
+        """evict_rows over every parameter, its state and `extra` (other [P, ...] tensors, e.g. max_radii2D): the groups hold new
+        Parameters afterwards, without gradients.  Returns (kept, scores, [extra])."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        names = [[k for k in ("exp_avg", "exp_avg_sq", "ratio") if k in self.state.get(p, {})] for p in params]
+        coded = [p for p in params if "rms" in self.state.get(p, {})]
+        rows = [p.detach() for p in params] + [self.state[p][k] for p, ks in zip(params, names) for k in ks] + list(extra)
+        kept, out, rows, pairs = evict_rows(scores, keep, rows, recent, weights, decay, [(self.state[p]["rms"], self.state[p]["window"]) for p in coded])
+        rest, pairs = iter(rows[len(params):]), dict(zip(map(id, coded), pairs))
+        for p, data, ks in zip(params, rows, names):
+            states = {k: next(rest) for k in ks}
+            if id(p) in pairs:
+                states["rms"], states["window"] = pairs[id(p)]
+            self._replace(p, data, states)
+        return kept, out, list(rest)
+
+    @torch.no_grad()
+    def append_rows(self, new):
+        """Adds rows to every parameter (cat_tensors_to_optimizer, gaussian_model.py:307-328): `new` is one tensor per parameter, in the groups'
+        order; the newcomers' moments are zero, the step counts go on.  The groups hold new Parameters afterwards, without gradients."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        if len(new) != len(params):
+            raise ValueError(f"append_rows: {len(new)} tensors for {len(params)} parameters")
+        for p, x in zip(params, new):
+            if x.shape[1:] != p.shape[1:] or x.dim() != p.dim():
+                raise ValueError(f"append_rows: rows of shape {tuple(x.shape)} for a parameter of shape {tuple(p.shape)}")
+        for p, x in zip(params, new):
+            data = torch.cat((p.detach(), x.detach().to(device=p.device, dtype=p.dtype)))
+            states = {}
+            for k, v in self.state.get(p, {}).items():
+                if k in ("exp_avg", "exp_avg_sq", "rms", "ratio"):
+                    states[k] = torch.cat((v, v.new_zeros(x.shape)))
+                elif k == "window":
+                    states[k] = torch.cat((v, v.new_zeros((data.numel() + WINDOW - 1) // WINDOW - v.numel())))
+            self._replace(p, data, states)

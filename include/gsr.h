@@ -476,6 +476,74 @@ int gsr_training_loss(int width, int height, const float* image, const float* gt
 int gsr_densification_stats(int P, const int* radii, const float* dL_dmean2D, float* max_radii2D,
                             float* xyz_gradient_accum, float* denom, void* stream);
 
+/* The optimiser step of a map (what gaussian_splatting/train.py:156-158 leaves to torch.optim.Adam: six tensors, a dozen launches
+ * each) and the pruning that goes with it (prune_points / _prune_optimizer, scene/gaussian_model.py:269-300).  Elements are dense;
+ * any number of tensors, of any sizes (zero included), in one call: 40 per launch.  No entry point here waits, reads anything back or
+ * uses memory beyond its arguments, so all of them can be captured into a graph; the step count lives on the device. */
+enum { GSR_TYPE_F32 = 0, GSR_TYPE_BF16 = 1, GSR_TYPE_F16 = 2 };
+
+/* Norm of the gradients over all tensors and the coefficient that clips it, as torch.nn.utils.clip_grad_norm_ defines them:
+ * out[0] = sqrt(sum g^2) (64-bit sums in a fixed order: the same bits every time), out[1] = min(1, max_norm / (out[0] + 1e-6)); a NaN
+ * stays one.  grads, numels, types: HOST arrays of n_tensors entries; workspace: callback for gsr_grad_norm_bytes(n_tensors) bytes. */
+size_t gsr_grad_norm_bytes(int n_tensors);
+int gsr_grad_norm(int n_tensors, const void* const* grads, const long long* numels, const int* types, float max_norm, float* out,
+                  gsr_resize_fn workspace, void* workspace_ctx, void* stream);
+
+/* One tensor of an AdamW step. */
+typedef struct gsr_opt_tensor {
+    void* param;                /* [n] of param_type, stepped in place */
+    const void* grad;           /* [n] of grad_type */
+    void* state0;               /* 32-bit moments: exp_avg f32 [n]; 8-bit: codes of sqrt(exp_avg_sq), uint8 [n] */
+    void* state1;               /* 32-bit: exp_avg_sq f32 [n]; 8-bit: codes of exp_avg / sqrt(exp_avg_sq), int8 [n] */
+    uint8_t* window;            /* 8-bit: uint8 [(n + 255) / 256]; otherwise unused */
+    double* clock;              /* f64 [4], this tensor's own: beta1^t, beta2^t, t, 0 -- before the first step 1, 1, 0, 0; advanced by the step */
+    const double* lr_device;    /* nullable: one f64 on the device instead of lr (a replayed graph reads it anew) */
+    double lr, weight_decay;
+    long long n;
+    int param_type, grad_type;  /* GSR_TYPE_* */
+} gsr_opt_tensor;
+typedef struct gsr_adamw_args {
+    int n_tensors;
+    int state_bits;             /* 32 or 8 */
+    const gsr_opt_tensor* tensors;      /* HOST array, read during the call only */
+    double beta1, beta2, eps;   /* 0 <= beta < 1; with 8 bits beta1^2 < beta2 too */
+    const float* clip;          /* nullable: gsr_grad_norm's out; the gradients count times clip[1] */
+    unsigned seed;              /* 8-bit: of the stochastic rounding (with the tensor's place in the list and the step) */
+    void* stream;
+} gsr_adamw_args;
+/* p <- p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)   with m <- beta1 m + (1 - beta1) g,
+ * v <- beta2 v + (1 - beta2) g^2 (torch.optim.AdamW; with weight_decay 0 torch.optim.Adam): computed in 32 bits, half-precision
+ * parameters rounded once.  With 8-bit moments the parameter is stepped with the moments before they are rounded; what is stored is
+ * described at k_adamw8 (csrc/gsr_mapopt.h).  Memory that a call writes must not overlap other memory of the call: refused. */
+int gsr_adamw_step(const gsr_adamw_args* args);
+/* The moments that 8-bit codes stand for: exp_avg[i], rms[i] = sqrt(exp_avg_sq)[i] of `type`, dense [n]. */
+typedef struct gsr_moment_tensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg_out; void* rms_out; long long n; } gsr_moment_tensor;
+int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream);
+
+/* One tensor that is compacted with the map: P rows of row_bytes bytes -> `keep` rows.  src_window (nullable): the tensor holds 8-bit
+ * root codes with these windows; dst_window gets the (keep * row_bytes + 255) / 256 windows of the result. */
+typedef struct gsr_row_tensor {
+    const void* src; void* dst;
+    const uint8_t* src_window; uint8_t* dst_window;
+    long long row_bytes;
+} gsr_row_tensor;
+typedef struct gsr_evict_args {
+    int P, n_views, keep, recent;       /* recent <= keep <= P */
+    const float* scores;        /* [P] accumulated so far */
+    const float* weights;       /* nullable if n_views = 0: [n_views, P], every splat's compositing weight in each view */
+    double decay;
+    long long* kept;            /* [keep] out: the rows that stay, ascending */
+    float* scores_out;          /* [keep] out: their accumulated weights */
+    int n_tensors;
+    const gsr_row_tensor* tensors;      /* HOST array, read during the call only */
+    gsr_resize_fn workspace; void* workspace_ctx;       /* gsr_evict_bytes(P) bytes */
+    void* stream;
+} gsr_evict_args;
+/* score = f32(decay * score + sum over views of weight) (64-bit sum); the last `recent` rows stay, and of the others the
+ * keep - recent with the largest score (ties: the lower index; NaN as -inf); every tensor's rows are copied in their order. */
+size_t gsr_evict_bytes(int P);
+int gsr_evict_rows(const gsr_evict_args* args);
+
 /* distCUDA2 (gaussian_splatting/submodules/simple-knn/simple_knn.cu:183-220 behind
  * spatial.cu:15-26): mean_dist2[i] = mean squared distance from point i to its three nearest OTHER points.
  * points [P,3], mean_dist2 [P] on the device; workspace: resize callback for gsr_knn_bytes(P) bytes. */

@@ -1,0 +1,748 @@
+"""-m gpu : the operators of gs_localization_amd.map_optimizer against 64-bit oracles (oracle/map_optimizer_oracle.py), at the sizes, types and
+values where they can go wrong.  Tolerances count roundings: e = 2^-24 for each 32-bit operation, half a step for a half-precision store."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import map_optimizer_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E = 2.0 ** -24
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+# sizes around a lane's four elements, a wave's 256, a workgroup's pass and its 4096
+SIZES = [1, 2, 3, 4, 5, 63, 64, 65, 255, 256, 257, 1023, 1025, 4095, 4096, 4097, 12289]
+
+
+def n64(t):
+    return t.detach().double().cpu().numpy().reshape(-1)
+
+
+def MO():
+    from gs_localization_amd import map_optimizer
+    return map_optimizer
+
+
+class Guarded:
+    """A tensor inside a larger allocation: `shift` elements behind its start, and what lies around it is watched."""
+
+    def __init__(self, values, shift=0):
+        n = values.numel()
+        self.buf = torch.full((n + shift + 64,), 93, dtype=values.dtype, device=DEV)
+        self.t = self.buf[shift:shift + n].view(values.shape)
+        self.t.copy_(values)
+        self.shift, self.n = shift, n
+
+    def check(self):
+        assert bool((self.buf[: self.shift] == 93).all()) and bool((self.buf[self.shift + self.n:] == 93).all()), "written outside of a tensor"
+
+
+def tensors32(sizes, gen, ptype, gtype, shift=0, step=3):
+    """Guarded (p, g, m, v) with gradients over four decades, a third of them zero, and moments that such gradients leave."""
+    out = []
+    for n in sizes:
+        mag = 10.0 ** (torch.rand(n, generator=gen, device=DEV) * 4 - (3 if gtype == torch.float16 else 6))
+        seen = torch.rand(n, generator=gen, device=DEV) < 0.67
+        p = torch.randn(n, generator=gen, device=DEV).to(ptype)
+        g = (torch.randn(n, generator=gen, device=DEV) * mag * seen).to(gtype)
+        u = mag * (0.2 + torch.rand(n, generator=gen, device=DEV)) if step else torch.zeros(n, device=DEV)
+        m = u * torch.randn(n, generator=gen, device=DEV) * 0.5
+        out.append([Guarded(x, shift) for x in (p, g, m, u * u)])
+    return out
+
+
+def clocks(k, t, betas):
+    return [torch.tensor([betas[0] ** t, betas[1] ** t, t, 0.0], dtype=torch.float64, device=DEV) for _ in range(k)]
+
+
+def bound32(p, m, v, scale, lr, decay, ptype, store=True):
+    """Roundings of one step.  v: two products' constants, products and a sum, all positive: 5 e.  sqrt (e, halves its argument's), times the
+    unbiasing factor (2 e), plus eps (2 e): 7.5 e on the denominator; m: 4 e of |m| b1 + |g| (1 - b1) with the clip's product 2 more; division, rate,
+    product: 3 e; so 17 e of the update's terms; p (1 - lr wd): 2 e, the difference e."""
+    tol = E * (17.5 * scale + 3.0 * np.abs(p) + scale)
+    return tol + HALF[ptype] * np.abs(p) + (2.0 ** -25 if ptype == torch.float16 else 2.0 ** -149) if store else tol
+
+
+def check32(before, after, t, lr, betas, eps, decay, coef, ptype):
+    p, g, m, v = (n64(x) for x in before)
+    p1, m1, v1, scale = O.adamw(p, g, m, v, t, lr, betas, eps, decay, coef)
+    got = [n64(x) for x in (after[0].t, after[2].t, after[3].t)]
+    assert (np.abs(got[1] - m1) <= 6 * E * (np.abs(m) * betas[0] + np.abs(g * coef) * (1 - betas[0])) + 2.0 ** -148).all()
+    assert (np.abs(got[2] - v1) <= 7 * E * v1 + 2.0 ** -147).all()
+    assert (np.abs(got[0] - p1) <= bound32(p1, m1, v1, scale, lr, decay, ptype)).all(), np.abs(got[0] - p1).max()
+
+
+@pytest.mark.parametrize("ptype, gtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                          (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("t, clip, decay", [(0, False, 0.0), (5, True, 0.01), (4000, True, 0.3)])
+def test_adamw32(ptype, gtype, shift, t, clip, decay):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    betas, eps, lr = (0.9, 0.999), 1e-15, 0.02
+    ts = tensors32(SIZES, gen, ptype, gtype, shift, step=t)
+    coef = float(np.float32(0.37)) if clip else 1.0
+    clip = torch.tensor([2.0, coef], device=DEV) if clip else None
+    ck = clocks(len(ts), t, betas)
+    for step in (1, 2):
+        before = [[x.t.clone() for x in q] for q in ts]
+        MO().adamw_step([q[0].t for q in ts], [q[1].t for q in ts], [q[2].t for q in ts], [q[3].t for q in ts], ck, lr=lr, betas=betas, eps=eps,
+                        weight_decay=decay, clip=clip)
+        for b, q in zip(before, ts):
+            check32(b, q, t + step, lr, betas, eps, decay, coef, ptype)
+            assert torch.equal(b[1], q[1].t)
+            for x in q:
+                x.check()
+        for c in ck:
+            assert c.tolist()[2:] == [t + step, 0.0] and abs(float(c[0]) - betas[0] ** (t + step)) < 1e-15 and abs(float(c[1]) - betas[1] ** (t + step)) < 1e-14
+
+
+@pytest.mark.parametrize("count", [1, 39, 40, 41, 130])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_tensors(count, bits):
+    """more tensors than a launch takes, empty ones among them, rates and decays of their own: each as if stepped alone"""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    sizes = [(7 * i * i + 13 * i) % 5000 if i % 5 else 0 for i in range(1, count + 1)]
+    lrs, wds = [0.001 * (i + 1) for i in range(count)], [0.01 * (i % 3) for i in range(count)]
+
+    def make():
+        g = torch.Generator(device=DEV).manual_seed(3)
+        return [[torch.randn(n, generator=g, device=DEV) for _ in range(2)] +
+                ([torch.zeros(n, device=DEV) for _ in range(2)] + [None] if bits == 32 else
+                 [torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros((n + 255) // 256, dtype=torch.uint8, device=DEV)])
+                for n in sizes]
+    a, b = make(), make()
+    ca, cb = clocks(count, 0, (0.9, 0.999)), clocks(count, 0, (0.9, 0.999))
+    col = lambda x, k: [r[k] for r in x]                                                       # noqa: E731
+    for _ in range(2):
+        if bits == 32:
+            MO().adamw_step(col(a, 0), col(a, 1), col(a, 2), col(a, 3), ca, lr=lrs, weight_decay=wds)
+            for i in range(count):
+                MO().adamw_step([b[i][0]], [b[i][1]], [b[i][2]], [b[i][3]], [cb[i]], lr=lrs[i], weight_decay=wds[i])
+        else:
+            MO().adamw_step_8bit(col(a, 0), col(a, 1), col(a, 2), col(a, 3), col(a, 4), ca, lr=lrs, weight_decay=wds, seed=5)
+            for i in range(count):          # (the place in the list is part of the seed: put the tensor at its place, behind empty ones)
+                e = [torch.zeros(0, device=DEV), torch.zeros(0, device=DEV), torch.zeros(0, dtype=torch.uint8, device=DEV), torch.zeros(0, dtype=torch.int8, device=DEV),
+                     torch.zeros(0, dtype=torch.uint8, device=DEV)]
+                rows = [e] * i + [b[i]]
+                MO().adamw_step_8bit(*[col(rows, k) for k in range(5)], clocks(i, 0, (0.9, 0.999)) + [cb[i]], lr=lrs[i], weight_decay=wds[i], seed=5)
+    for x, y, u, w in zip(a, b, ca, cb):
+        assert torch.equal(u, w)
+        for k in range(5):
+            assert x[k] is None or torch.equal(x[k], y[k])
+
+
+def random_codes(n, gen, shift=0, low=60, high=120):
+    window = torch.randint(low, high, ((n + 255) // 256,), generator=gen, device=DEV).to(torch.uint8)
+    rms = torch.randint(0, 256, (n,), generator=gen, device=DEV).to(torch.uint8)
+    ratio = torch.randint(-127, 128, (n,), generator=gen, device=DEV).to(torch.int8)
+    ratio.masked_fill_(rms == 0, 0)
+    return Guarded(rms, shift), Guarded(ratio, shift), Guarded(window, shift)
+
+
+def check8(before, after, place, t, lr, betas, eps, decay, coef, seed, ptype):
+    """The stored codes are floors of fractional places: they may differ from the oracle's only where its place lies within the 32-bit
+    computation's error of a whole number, and then by one."""
+    p, g, rms, ratio, window = before
+    p1, m1, u1, at, dr, scale = O.adamw8(n64(p), n64(g), rms.cpu().numpy(), ratio.cpu().numpy(), window.cpu().numpy(), t, lr, betas, eps, decay, coef, seed, place)
+    n = p1.size
+    # as with 32 bits, the moments decoded with 2 e more
+    assert (np.abs(n64(after[0].t) - p1) <= bound32(p1, m1, None, scale * 1.2, lr, decay, ptype)).all()
+    got_w = after[4].t.cpu().numpy().astype(np.int64)
+    big = np.floor(O.grid_place(u1)).astype(np.int64)
+    want_w = O.window_of(big)
+    # the window: of a largest root within 6 e of the next binade, that binade's
+    assert (got_w == want_w).all() or (np.abs(got_w - want_w) <= (np.abs(O.grid_place(u1 * (1 + 8 * E)) // 16 - O.grid_place(u1 * (1 - 8 * E)) // 16).max())).all()
+    codes = after[2].t.cpu().numpy().astype(np.int64).reshape(-1)
+    place_got = np.where(codes > 0, codes + 16 * O.per_block(got_w, n) + 1, 0)
+    low = 16 * O.per_block(got_w, n) + 2
+    want = np.where(u1 > 0, np.maximum(np.floor(at), low), 0)
+    tol_u = 32 * 6 * E * 1.01 + 1e-9          # a relative error of 6 e moves a root by at most 32 sixteenths of its binade times that
+    frac = at - np.floor(at)
+    near = (np.minimum(frac, 1 - frac) <= tol_u)
+    assert (place_got[~near] == want[~near]).all() and (np.abs(place_got - want)[near] <= 1).all()
+    assert near.mean() < 1e-3 or n < 5000
+    assert (codes[u1 == 0] == 0).all()
+    uq = O.decode(codes, got_w)
+    r = np.divide(m1, uq, out=np.zeros(n), where=uq > 0) * 127 / O.span(*betas) + dr
+    wr = np.where(uq > 0, np.clip(np.floor(r), -127, 127), 0)
+    gr = after[3].t.cpu().numpy().astype(np.int64).reshape(-1)
+    # m: 8 e of its terms' size (they may cancel), the quotient and the constant 4 e, the sum's rounding e of its size
+    size = np.divide(np.abs(n64(ratio)) / 127 * O.span(*betas) * O.decode(rms.cpu().numpy(), window.cpu().numpy()) * betas[0] + np.abs(n64(g) * coef) * (1 - betas[0]),
+                     uq, out=np.zeros(n), where=uq > 0) * 127 / O.span(*betas)
+    tol_r = E * (14 * size + 2 * np.abs(r) + 2)
+    near = np.abs(r - np.rint(r)) <= tol_r
+    assert (gr[~near] == wr[~near]).all() and (np.abs(gr - wr)[near] <= 1).all()
+    assert near.mean() < 2e-2 or n < 5000
+
+
+@pytest.mark.parametrize("ptype, gtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("t, clip, decay", [(0, False, 0.0), (17, True, 0.01)])
+def test_adamw8(ptype, gtype, shift, t, clip, decay):
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    betas, eps, lr, seed = (0.9, 0.999), 1e-15, 0.02, 12345
+    coef = float(np.float32(0.37)) if clip else 1.0
+    clip = torch.tensor([2.0, coef], device=DEV) if clip else None
+    ts = []
+    for n in SIZES:
+        low, high = (95, 105) if gtype == torch.float16 else (60, 120)
+        rms, ratio, window = random_codes(n, gen, shift, low, high)
+        g = torch.randn(n, generator=gen, device=DEV) * torch.exp2(window.t.float() - 120.0).repeat_interleave(256)[:n] * 10.0 ** (torch.rand(n, generator=gen, device=DEV) * 2)
+        g *= torch.rand(n, generator=gen, device=DEV) < 0.7
+        if t == 0:
+            for x in (rms, ratio, window):
+                x.t.zero_()
+        ts.append([Guarded(torch.randn(n, generator=gen, device=DEV).to(ptype), shift), Guarded(g.to(gtype), shift), rms, ratio, window])
+    ck = clocks(len(ts), t, betas)
+    for step in (1, 2, 3):
+        before = [[x.t.clone() for x in q] for q in ts]
+        MO().adamw_step_8bit(*[[q[k].t for q in ts] for k in range(5)], ck, lr=lr, betas=betas, eps=eps, weight_decay=decay, clip=clip, seed=seed)
+        for i, (b, q) in enumerate(zip(before, ts)):
+            check8(b, q, i, t + step, lr, betas, eps, decay, coef, seed, ptype)
+            for x in q:
+                x.check()
+    avg, root = MO().moments_8bit([q[2].t for q in ts], [q[3].t for q in ts], [q[4].t for q in ts])
+    for q, a, r in zip(ts, avg, root):
+        u = O.decode(q[2].t.cpu().numpy(), q[4].t.cpu().numpy())
+        assert (n64(r) == u).all()
+        m = n64(q[3].t) / 127 * O.span(*betas) * u
+        assert (np.abs(n64(a) - m) <= 3 * E * np.abs(m) + 2.0 ** -149).all()          # the unit's rounding and two products
+
+
+def test_adamw8_mean_follows_32_bits():
+    """What the bytes stand for is the 32-bit moments on average: 4096 equal elements, 300 steps with gradients of changing size (beta2 = 0.999: a rounding
+    to the nearest sixteenth would stand still).  A root's stochastic step is at most 1/16 of it and moves by the change (0.0005) only: each step adds
+    at most 0.0005 / 16 to the relative variance; 300 steps, four more for the drift of u^2 against v (f (1 - f) step^2), five standard errors over 4096."""
+    n = 4096
+    p = [torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)]
+    m, v = [torch.zeros(n, device=DEV) for _ in range(2)]
+    rms, ratio, window = torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros(n // 256, dtype=torch.uint8, device=DEV)
+    ca, cb = clocks(1, 0, (0.9, 0.999)), clocks(1, 0, (0.9, 0.999))
+    for k in range(300):
+        g = torch.full((n,), 1e-5 * (3.0 if k > 150 else 1.0) * (1 if k % 3 else -1), device=DEV)
+        MO().adamw_step([p[0]], [g], [m], [v], ca, lr=1e-3, eps=1e-15)
+        MO().adamw_step_8bit([p[1]], [g], [rms], [ratio], [window], cb, lr=1e-3, eps=1e-15, seed=1)
+    (avg,), (root,) = MO().moments_8bit([rms], [ratio], [window])
+    drift = 300 * 0.0005 / 16
+    assert abs(float(root.double().mean() / v.double().sqrt().mean()) - 1) < 4 * drift + 5 * math.sqrt(300 * 0.0005 / 16 / n)
+    assert abs(float((avg.double().mean() - m.double().mean()) / v.double().sqrt().mean())) < O.span(0.9, 0.999) / 127 * 5 / math.sqrt(n) * math.sqrt(10) + 4 * drift * 0.5
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 1e30])
+def test_one_bad_gradient_stays_alone(bad):
+    """32 bits: torch's values.  8 bits: the element's neighbours step and round as if it were not there."""
+    n = 700
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    g = torch.randn(n, generator=gen, device=DEV)
+    out = {}
+    for name, x in (("good", g[300].item()), ("bad", bad)):
+        gg = g.clone()
+        gg[300] = x
+        p = torch.ones(n, device=DEV)
+        rms, ratio, window = torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros(3, dtype=torch.uint8, device=DEV)
+        ck = clocks(1, 0, (0.9, 0.999))
+        for _ in range(2):
+            MO().adamw_step_8bit([p], [gg], [rms], [ratio], [window], ck, lr=0.1, seed=3)
+        q, m, v = torch.ones(n, device=DEV), torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+        MO().adamw_step([q], [gg], [m], [v], clocks(1, 0, (0.9, 0.999)), lr=0.1)
+        out[name] = (p, rms, ratio, window, q, m, v)
+    others = torch.arange(n, device=DEV) != 300
+    for k in (0, 4, 5, 6):
+        assert torch.equal(out["good"][k][others], out["bad"][k][others])
+    for k in (1, 2):
+        assert torch.equal(out["good"][k][others], out["bad"][k][others])
+    assert torch.equal(out["good"][3], out["bad"][3]) or abs(float(g[300])) >= float(g[256:512].abs().max())
+    q, m = out["bad"][4][300].item(), out["bad"][5][300].item()
+    ref = torch.ones(1, dtype=torch.float32, requires_grad=True)
+    ref.grad = torch.tensor([bad])
+    torch.optim.Adam([ref], lr=0.1).step()
+    ref = ref.detach()
+    assert (math.isnan(q) and math.isnan(float(ref))) or q == pytest.approx(float(ref), rel=1e-6)
+    assert math.isnan(m) == math.isnan(bad)
+
+
+def test_extreme_sizes_of_gradients():
+    """Denormal squares, all-zero blocks, a block over more than sixteen binades, and a root near the largest float: no NaN, windows at their ends."""
+    cases = dict(tiny=torch.full((256,), 1e-22), zero=torch.zeros(256), wide=10.0 ** torch.linspace(-18, 0, 256), huge=torch.full((256,), 1e19), one=torch.eye(16).reshape(-1))
+    for name, g in cases.items():
+        g = g.to(DEV)
+        p = torch.ones(256, device=DEV)
+        rms, ratio, window = torch.zeros(256, dtype=torch.uint8, device=DEV), torch.zeros(256, dtype=torch.int8, device=DEV), torch.zeros(1, dtype=torch.uint8, device=DEV)
+        ck = clocks(1, 0, (0.9, 0.999))
+        for t in (1, 2, 3):
+            before = [x.clone() for x in (p, g, rms, ratio, window)]
+            MO().adamw_step_8bit([p], [g], [rms], [ratio], [window], ck, lr=0.01, eps=1e-15, seed=9)
+            assert bool(p.isfinite().all())
+            if name in ("wide", "one", "zero"):
+                after = [type("G", (), dict(t=x)) for x in (p, g, rms, ratio, window)]
+                check8(before, after, 0, t, 0.01, (0.9, 0.999), 1e-15, 0.0, 1.0, 9, torch.float32)
+        # an update is at most lr times the ratio's range, unbiased: 7.27 sqrt(1 - b2^t) / (1 - b1^t), less than 1.3 in the first three steps
+        assert float((p - 1).abs().max()) <= 3 * 0.01 * 1.3 + 1e-6, name
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_counts_on(bits):
+    """A captured step replays like eager ones: the clock and a rate on the device are read anew each time."""
+    def make():
+        gen = torch.Generator(device=DEV).manual_seed(7)
+        ps = [torch.nn.Parameter(torch.randn(n, generator=gen, device=DEV)) for n in (3, 1000, 5000)]
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+        lr = torch.tensor(0.01, dtype=torch.float64, device=DEV)
+        return ps, lr, MO().AdamW(ps, lr=lr, eps=1e-15, state_bits=bits, max_norm=3.0, weight_decay=0.01, seed=4)
+    (pa, la, oa), (pb, lb, ob) = make(), make()
+    oa.step(); ob.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        oa.step()
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(4):
+        for p, q in zip(pa, pb):
+            noise = torch.randn(p.shape, device=DEV)
+            p.grad.copy_(noise); q.grad.copy_(noise)
+        la.fill_(0.01 / (k + 1)); lb.fill_(0.01 / (k + 1))
+        graph.replay()
+        ob.step()
+        torch.cuda.synchronize()
+        for p, q in zip(pa, pb):
+            assert torch.equal(p, q)
+            for key in ob.state[q]:
+                assert torch.equal(oa.state[p][key], ob.state[q][key])
+        assert float(oa.state[pa[0]]["step"][2]) == k + 2
+        assert torch.equal(oa.last_norm, ob.last_norm)
+
+
+def test_first_step_is_not_captured():
+    p = torch.nn.Parameter(torch.zeros(8, device=DEV))
+    p.grad = torch.ones(8, device=DEV)
+    opt = MO().AdamW([p])
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+
+
+def test_other_stream_and_versions():
+    p = torch.nn.Parameter(torch.ones(100_000, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = MO().AdamW([p], lr=0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            opt.step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert float((p.detach() - 0.7).abs().max()) < 1e-5
+    loss = (p * p).sum()          # saved for backward, then stepped: autograd must notice
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_gradients_with_strides_and_refused_layouts():
+    g = torch.randn(6, 8, device=DEV)
+    state = lambda: (torch.zeros(8, 6, device=DEV), torch.zeros(8, 6, device=DEV), clocks(1, 0, (0.9, 0.999))[0])       # noqa: E731
+    outs = []
+    for grad in (g.t(), g.t().contiguous()):
+        p = torch.ones(8, 6, device=DEV)
+        m, v, c = state()
+        MO().adamw_step([p], [grad], [m], [v], [c], lr=0.1)
+        outs.append(p)
+    assert torch.equal(*outs)
+    p, (m, v, c) = torch.ones(8, 6, device=DEV), state()
+    MO().adamw_step([p], [torch.ones(1, device=DEV).expand(8, 6)], [m], [v], [c], lr=0.1)
+    assert float((p - 0.9).abs().max()) < 1e-6
+    m, v, c = state()
+    ok = dict(params=[p], grads=[p.clone()], exp_avgs=[m], exp_avg_sqs=[v], clocks=[c], lr=0.1)
+    for change, err in ((dict(params=[torch.ones(6, 8, device=DEV).t()]), ValueError), (dict(params=[p.double()], grads=[p.double()]), TypeError),
+                        (dict(grads=[torch.ones(48, device=DEV)]), ValueError), (dict(exp_avgs=[m.bfloat16()]), TypeError), (dict(exp_avgs=[m[:4]]), ValueError),
+                        (dict(clocks=[c.float()]), TypeError), (dict(clocks=[c[:3]]), ValueError), (dict(clip=torch.ones(1, device=DEV)), ValueError),
+                        (dict(lr=[torch.tensor(0.1, device=DEV)]), ValueError), (dict(exp_avgs=[v]), RuntimeError), (dict(grads=[p]), RuntimeError)):
+        with pytest.raises(err):
+            MO().adamw_step(**dict(ok, **change))
+    assert float(c[2]) == 0.0
+
+
+def test_empty_tensors():
+    p = [torch.zeros(0, 3, device=DEV), torch.zeros(5, 0, 3, device=DEV)]
+    z = lambda: [torch.zeros_like(x) for x in p]                                               # noqa: E731
+    ck = clocks(2, 0, (0.9, 0.999))
+    MO().adamw_step(p, z(), z(), z(), ck, lr=0.1)
+    assert [float(c[2]) for c in ck] == [1.0, 1.0]
+    assert MO().grad_norm(z(), 1.0).tolist() == [0.0, 1.0]
+    MO().adamw_step([], [], [], [], [], lr=0.1)
+
+
+# ---- the norm ----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5], SIZES, [100_000, 1, 777_777], [17] * 500, [0]])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_grad_norm(sizes, dtype, shift):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    gs = [Guarded((torch.randn(n, generator=gen, device=DEV) * 3).to(dtype), shift).t for n in sizes]
+    for max_norm in (0.0, 1.0, 1e9, math.inf):
+        out = MO().grad_norm(gs, max_norm)
+        n, c = O.norm([n64(g) for g in gs], max_norm)
+        got = out.double().tolist()
+        # the 64-bit sum is off by at most (elements per partial sum + partial sums) 2^-53 of itself, the result by one 32-bit rounding
+        assert abs(got[0] - n) <= (E + 1e-9) * n
+        assert abs(got[1] - c) <= 4 * E * c or (got[1] == 1.0 and c > 1 - 4 * E)
+        assert torch.equal(out, MO().grad_norm(gs, max_norm))
+    assert not any(bool((g != g).any()) for g in gs)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_grad_norm_not_finite(bad):
+    g = torch.ones(10_000, device=DEV)
+    g[5000] = bad
+    n, c = MO().grad_norm([torch.ones(3, device=DEV), g], 1.0).tolist()
+    ref = torch.ones(10_000, requires_grad=True)
+    ref.grad = g.cpu()
+    want = float(torch.nn.utils.clip_grad_norm_([ref], 1.0))
+    assert (math.isnan(n) and math.isnan(want)) or n == want
+    assert math.isnan(c) if math.isnan(bad) else c == 0.0
+
+
+def test_norm_does_not_overflow_or_vanish():
+    for x in (1e-30, 1e25):
+        n, _ = MO().grad_norm([torch.full((1000,), x, device=DEV)], 1.0).double().tolist()
+        x = float(np.float32(x))
+        assert abs(n - x * math.sqrt(1000)) <= 2 * E * n
+
+
+# ---- eviction ----------------------------------------------------------------------------------------------------------------------
+
+def evict_inputs(P, gen, kind):
+    s = torch.rand(P, generator=gen, device=DEV) * 5
+    if kind == "ties":
+        s = torch.randint(0, 3, (P,), generator=gen, device=DEV).float()
+    elif kind == "equal":
+        s = torch.full((P,), 0.25, device=DEV)
+    elif kind == "odd":
+        pool = torch.tensor([0.0, -0.0, 1e-45, -1e-45, float("nan"), float("inf"), -float("inf"), 1.0, -1.0, 3.4e38, -3.4e38, -float("nan")], device=DEV)
+        s = pool[torch.randint(0, len(pool), (P,), generator=gen, device=DEV)]
+    return s
+
+
+@pytest.mark.parametrize("P", [1, 2, 63, 64, 255, 256, 257, 1023, 1024, 1025, 4096, 5000, 70_001, 300_000])
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "odd"])
+def test_evict_rows(P, kind):
+    gen = torch.Generator(device=DEV).manual_seed(P)
+    s = evict_inputs(P, gen, kind)
+    tensors = [torch.randn(P, 3, generator=gen, device=DEV), torch.randn(P, 1, 3, generator=gen, device=DEV), torch.randn(P, generator=gen, device=DEV).bfloat16(),
+               torch.randn(P, 3, generator=gen, device=DEV).half(), torch.rand(P, generator=gen, device=DEV) < 0.5, torch.randint(0, 99, (P, 5), generator=gen, device=DEV),
+               torch.randn(P, 4, generator=gen, device=DEV), torch.zeros(P, 0, 3, device=DEV), torch.randint(0, 99, (P, 7), generator=gen, device=DEV).to(torch.uint8),
+               torch.randn(3, P, generator=gen, device=DEV).t(), torch.randn(P * 3 + 1, generator=gen, device=DEV)[1:].view(P, 3)]
+    for keep, recent, views, decay in ((P, 0, 0, 1.0), (0, 0, 1, 1.0), (1, 0, 2, 0.5), (P // 2, 0, 0, 1.0), ((P + 1) // 2, P // 4, 3, 0.9), (P - 1, P // 2, 1, 1.0),
+                                       (P // 3, P // 3, 1, 1.0), (P, P, 0, 1.0), (max(1, P - 1), 1, 2, 0.0)):
+        recent = min(recent, keep)
+        w = torch.rand(views, P, generator=gen, device=DEV) if views else None
+        kept, scores, rows, _ = MO().evict_rows(s, keep, tensors, recent=recent, weights=w, decay=decay)
+        want, ws = O.evict(s.cpu().numpy(), keep, recent, None if w is None else w.cpu().numpy(), decay)
+        assert kept.dtype == torch.int64 and np.array_equal(kept.cpu().numpy(), want), (P, kind, keep, recent)
+        assert np.array_equal(scores.cpu().numpy(), ws, equal_nan=True)
+        for x, y in zip(tensors, rows):
+            assert y.dtype == x.dtype and y.shape == (keep, *x.shape[1:]) and torch.equal(y, x[kept])
+
+
+def test_evict_many_tensors_and_wide_rows():
+    P = 3000
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    s = torch.rand(P, generator=gen, device=DEV)
+    tensors = [torch.randn(P, 1 + (i * 37) % 90, generator=gen, device=DEV) for i in range(90)] + [torch.randn(P, 70_001, generator=gen, device=DEV)]
+    kept, _, rows, _ = MO().evict_rows(s, 1234, tensors)
+    for x, y in zip(tensors, rows):
+        assert torch.equal(x[kept], y)
+
+
+@pytest.mark.parametrize("P, width", [(1, 1), (5, 3), (85, 3), (86, 3), (3000, 1), (3000, 45), (777, 256), (40, 300)])
+def test_evict_recodes_8_bit_roots(P, width):
+    """A row's codes move into their new block's window: the same values, or that window's lowest."""
+    gen = torch.Generator(device=DEV).manual_seed(P + width)
+    n = P * width
+    for low, high in ((100, 104), (60, 120)):
+        rms, ratio, window = (x.t for x in random_codes(n, gen, 0, low, high))
+        s = torch.rand(P, generator=gen, device=DEV)
+        keep = (2 * P + 2) // 3
+        kept, _, (r2,), ((c2, w2),) = MO().evict_rows(s, keep, [ratio.view(P, width)], rms=[(rms.view(P, width), window)])
+        u = O.decode(rms.cpu().numpy(), window.cpu().numpy()).reshape(P, width)[kept.cpu().numpy()].reshape(-1)
+        w = O.window_of(np.rint(O.grid_place(u)).astype(np.int64))
+        assert np.array_equal(w2.cpu().numpy(), w) and np.array_equal(c2.cpu().numpy().reshape(-1), O.recode(u, w))
+        assert torch.equal(r2, ratio.view(P, width)[kept])
+        if high - low < 16 - 8:          # windows four apart: only the lowest few codes can fall under
+            back = O.decode(c2.cpu().numpy(), w2.cpu().numpy())
+            assert (back >= u).all() and (back[c2.cpu().numpy().reshape(-1) > 1] == u[c2.cpu().numpy().reshape(-1) > 1]).all()
+
+
+def test_offsets_past_32_bits():
+    """more than 2^31 elements in a tensor, and rows that lie more than 2^32 bytes into theirs"""
+    n = (1 << 31) + 12_345
+    look = [slice(0, 5000), slice((1 << 31) - 3000, (1 << 31) + 3000), slice(n - 5000, n)]
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    for s in look:
+        p[s] = torch.randn(s.stop - s.start, device=DEV).bfloat16()
+        g[s] = torch.randn(s.stop - s.start, device=DEV).bfloat16()
+    rms, ratio, window = torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros((n + 255) // 256, dtype=torch.uint8, device=DEV)
+    before = [p[s].clone() for s in look]
+    MO().adamw_step_8bit([p], [g], [rms], [ratio], [window], clocks(1, 0, (0.9, 0.999)), lr=0.1, seed=1)
+    betas = (0.9, 0.999)
+    for s, b in zip(look, before):
+        p1, m1, v1, scale = O.adamw(n64(b), n64(g[s]), 0, 0, 1, 0.1, betas, 1e-8, 0.0)
+        assert (np.abs(n64(p[s]) - p1) <= bound32(p1, m1, v1, scale, 0.1, 0.0, torch.bfloat16)).all()
+        du, _ = O.dither(np.arange(s.start, s.stop), 1, 0, 1)
+        first = s.start // 256
+        win = window[first:(s.stop + 255) // 256].cpu().numpy().astype(np.int64)
+        codes = rms[s].cpu().numpy().astype(np.int64)
+        w = np.repeat(win, 256)[s.start - first * 256:][: codes.size]
+        at = O.grid_place(np.sqrt(v1)) + du / 2.0 ** 19
+        got = np.where(codes > 0, codes + 16 * w + 1, 0)
+        near = np.abs(at - np.rint(at)) < 1e-4
+        want = np.where(v1 > 0, np.maximum(np.floor(at), 16 * w + 2), 0)
+        assert (got[~near] == want[~near]).all()
+    norm = float(MO().grad_norm([g], 1.0)[0])
+    want = math.sqrt(sum(float((n64(g[s]) ** 2).sum()) for s in look))
+    assert abs(norm - want) <= 2 * E * want
+    del rms, ratio, window
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    before = [p[s].clone() for s in look]
+    MO().adamw_step([p], [g], [m], [v], clocks(1, 0, (0.9, 0.999)), lr=0.1)
+    for s, b in zip(look, before):
+        p1, m1, v1, scale = O.adamw(n64(b), n64(g[s]), 0, 0, 1, 0.1, betas, 1e-8, 0.0)
+        assert (np.abs(n64(p[s]) - p1) <= bound32(p1, m1, v1, scale, 0.1, 0.0, torch.bfloat16)).all()
+        assert (np.abs(n64(v[s]) - v1) <= 7 * E * v1).all()
+    del m, v, p, g
+    torch.cuda.empty_cache()
+    P, width = 1_300_000, 1001          # 5.2 GB of 4-byte units
+    x = torch.empty(P, width, device=DEV)
+    x[:] = torch.arange(P, device=DEV, dtype=torch.float32)[:, None]
+    x[:, 7] += 0.5
+    s = torch.zeros(P, device=DEV)
+    s[P - 1000:] = 1.0
+    s[:3] = 2.0
+    kept, _, (y,), _ = MO().evict_rows(s, 1_200_000, [x])
+    assert kept[:3].tolist() == [0, 1, 2] and kept[-1000:].tolist() == list(range(P - 1000, P))
+    assert torch.equal(y[-1500:], x[kept[-1500:]]) and torch.equal(y[600_000:600_100], x[kept[600_000:600_100]])
+
+
+# ---- the optimiser ------------------------------------------------------------------------------------------------------------------
+
+def small_map(P, gen, bits, **kw):
+    shapes = dict(xyz=(P, 3), f_dc=(P, 1, 3), f_rest=(P, 3, 3), opacity=(P, 1), scaling=(P, 3), rotation=(P, 4))
+    ps = {k: torch.nn.Parameter(torch.randn(s, generator=gen, device=DEV)) for k, s in shapes.items()}
+    return ps, MO().AdamW([{"params": [p], "lr": 0.01 * (i + 1), "name": k} for i, (k, p) in enumerate(ps.items())], lr=0.0, eps=1e-15, state_bits=bits, **kw)
+
+
+def fill_grads(opt, gen):
+    for g in opt.param_groups:
+        for p in g["params"]:
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+
+
+def test_optimizer_follows_torchs():
+    """Five steps beside torch.optim.Adam in 64 bits from the same gradients.  An error in m or v feeds on at b1 or b2 < 1, so it stays under its one
+    step's over (1 - b1): 40 e of the update's size (at most 1.3 lr per step here), five steps of it."""
+    gen = torch.Generator(device=DEV).manual_seed(20)
+    ps, opt = small_map(500, gen, 32, max_norm=1.0)
+    qs = [torch.nn.Parameter(p.detach().double().cpu()) for p in ps.values()]
+    ref = torch.optim.Adam([{"params": [q], "lr": 0.01 * (i + 1)} for i, q in enumerate(qs)], lr=0.0, eps=1e-15)
+    for _ in range(5):
+        fill_grads(opt, gen)
+        for p, q in zip(ps.values(), qs):
+            q.grad = p.grad.double().cpu()
+        torch.nn.utils.clip_grad_norm_(qs, 1.0)
+        opt.step(); ref.step()
+    for i, (p, q) in enumerate(zip(ps.values(), qs)):
+        assert (np.abs(n64(p) - n64(q)) <= E * (5 * 40 * 1.3 * 10 * 0.01 * (i + 1) + 15 * np.abs(n64(q)))).all()
+
+
+def test_parameter_without_gradient_is_skipped():
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    ps, opt = small_map(50, gen, 32)
+    fill_grads(opt, gen)
+    ps["opacity"].grad = None
+    before = ps["opacity"].detach().clone()
+    opt.step()
+    assert torch.equal(before, ps["opacity"]) and ps["opacity"] not in opt.state and float(opt.state[ps["xyz"]]["step"][2]) == 1.0
+    opt.zero_grad()
+    opt.step()
+    assert float(opt.state[ps["xyz"]]["step"][2]) == 1.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(bits):
+    gen = torch.Generator(device=DEV).manual_seed(22)
+    ps, opt = small_map(300, gen, bits)
+    fill_grads(opt, gen)
+    opt.step()
+    saved = opt.state_dict()
+    saved = dict(saved, state={i: {k: v.cpu().clone() for k, v in s.items()} for i, s in saved["state"].items()})
+    qs, opt2 = small_map(300, gen, bits)
+    with torch.no_grad():
+        for p, q in zip(ps.values(), qs.values()):
+            q.copy_(p)
+    opt2.load_state_dict(saved)
+    for p, q in zip(ps.values(), qs.values()):
+        p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+        q.grad = p.grad.clone()
+    opt.step(); opt2.step()
+    for p, q in zip(ps.values(), qs.values()):
+        assert torch.equal(p, q)
+        for k in opt.state[p]:
+            assert opt.state[p][k].dtype == opt2.state[q][k].dtype and torch.equal(opt.state[p][k], opt2.state[q][k])
+    if bits == 8:
+        with pytest.raises(ValueError, match="8-bit"):
+            opt.load_state_dict(small_trained_adam(300, gen))
+
+
+def small_trained_adam(P, gen):
+    ps, _ = small_map(P, gen, 32)
+    ref = torch.optim.Adam([{"params": [p], "lr": 0.01 * (i + 1), "name": k} for i, (k, p) in enumerate(ps.items())], lr=0.0, eps=1e-15)
+    for p in ps.values():
+        p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+    ref.step()
+    return ref.state_dict()
+
+
+def test_takes_torchs_state():
+    gen = torch.Generator(device=DEV).manual_seed(23)
+    ps, opt = small_map(100, gen, 32)
+    opt.load_state_dict(small_trained_adam(100, gen))
+    assert opt.state[ps["xyz"]]["step"].tolist() == [0.9, 0.999, 1.0, 0.0]
+    fill_grads(opt, gen)
+    opt.step()
+    assert float(opt.state[ps["xyz"]]["step"][2]) == 2.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_evict_and_append_keep_the_state_with_its_rows(bits):
+    gen = torch.Generator(device=DEV).manual_seed(24)
+    P = 1000
+    ps, opt = small_map(P, gen, bits)
+    fill_grads(opt, gen)
+    opt.step()
+    old = {g["name"]: (g["params"][0].detach().clone(), {k: v.clone() for k, v in opt.state[g["params"][0]].items()}) for g in opt.param_groups}
+    extra = torch.arange(P, device=DEV)
+    kept, _, (ex,) = opt.evict(torch.rand(P, generator=gen, device=DEV), 700, recent=50, extra=[extra])
+    assert torch.equal(ex, kept) and kept[-50:].tolist() == list(range(950, 1000))
+
+    def moments(st):
+        if bits == 32:
+            return st["exp_avg"], st["exp_avg_sq"]
+        (m,), (u,) = MO().moments_8bit([st["rms"]], [st["ratio"]], [st["window"]])
+        return m, u
+    for g in opt.param_groups:
+        p, (q, st) = g["params"][0], old[g["name"]]
+        assert isinstance(p, torch.nn.Parameter) and p.grad is None and p.requires_grad and torch.equal(p, q[kept])
+        assert set(opt.state[p]) == set(st) and torch.equal(opt.state[p]["step"], st["step"])
+        for a, b in zip(moments(opt.state[p]), moments(st)):          # gradients of one size: every root lies within its new window
+            assert torch.equal(a, b[kept])
+    assert len(opt.state) == 6
+    opt.append_rows([torch.ones((30, *g["params"][0].shape[1:]), device=DEV) for g in opt.param_groups])
+    for g in opt.param_groups:
+        p, (q, st) = g["params"][0], old[g["name"]]
+        assert p.shape[0] == 730 and torch.equal(p[:700], q[kept]) and bool((p[700:] == 1).all())
+        for a, b in zip(moments(opt.state[p]), moments(st)):
+            assert torch.equal(a[:700], b[kept]) and not bool(a[700:].any())
+    fill_grads(opt, gen)
+    opt.step()
+    with pytest.raises(ValueError, match="append_rows"):
+        opt.append_rows([torch.ones(3, 3, device=DEV)])
+
+
+def test_compositing_weights_of_the_rasterizer():
+    """The weights sum to what the picture's opacity says, and are those of a white splat's own picture."""
+    from tests import util as U  # noqa: F401
+    from gs_localization_amd import scenes as S
+    import diff_gaussian_rasterization as A
+    sc = S.small(P=400, W=96, H=64, sh_degree=1, seed=3, scale_med=0.08)
+    t = lambda a: torch.tensor(np.ascontiguousarray(a), dtype=torch.float32, device=DEV)          # noqa: E731
+    view, proj, _, campos = S.camera_matrices(sc, np.eye(4))
+    rs = A.GaussianRasterizationSettings(image_height=sc.H, image_width=sc.W, tanfovx=sc.tanfovx, tanfovy=sc.tanfovy, bg=torch.zeros(3, device=DEV), scale_modifier=1.0,
+                                         viewmatrix=t(view), projmatrix=t(proj), sh_degree=1, campos=t(campos), prefiltered=False, debug=False)
+    args = dict(means3D=t(sc.means3D), opacities=t(sc.opacities), scales=t(sc.scales), rotations=t(sc.rotations))
+    w = MO().compositing_weights(rs, **args)
+    with torch.no_grad():
+        image, _, _, alpha = A.GaussianRasterizer(rs)(means2D=torch.zeros(400, 3, device=DEV), colors_precomp=torch.ones(400, 3, device=DEV), **args)
+        # sums of some 10^5 positive terms in 32 bits, in any order: a pixel's alpha and its weights' sum agree to 1e-5, and so do the totals
+        assert float(w.double().sum()) == pytest.approx(float(alpha.double().sum()), rel=1e-4)
+        assert float(w.double().sum()) == pytest.approx(float(image[0].double().sum()), rel=1e-4)
+        best = int(w.argmax())
+        one = torch.zeros(400, 3, device=DEV)
+        one[best] = 1.0
+        image, *_ = A.GaussianRasterizer(rs)(means2D=torch.zeros(400, 3, device=DEV), colors_precomp=one, **args)
+        assert float(image[0].double().sum()) == pytest.approx(float(w[best]), rel=1e-4)
+    assert bool((w >= 0).all()) and w.shape == (400,)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_with_clipping_eviction_and_growth(bits):
+    """train.py's loop as a user of these operators runs it: render, loss, backward, clipped step; weights accumulated over views; the map pruned to a
+    budget, grown, and trained on.  With 32 bits every step is the oracle's on the gradients that the rasterizer gave."""
+    from tests.train_replay import TrainReplay, LRS
+    tr = TrainReplay(P0=5000, P1=5000, W=160, H=112, n_views=4, densify_from=10 ** 9)
+    opt = tr.opt = MO().AdamW([{"params": [tr.par[k]], "lr": LRS[k], "name": k} for k in LRS], lr=0.0, eps=1e-15, state_bits=bits, max_norm=0.01, seed=3)
+    for it in range(1, 5):
+        before = {k: v.detach().clone() for k, v in tr.par.items()}
+        state = {k: {x: y.clone() for x, y in opt.state[v].items()} for k, v in tr.par.items() if v in opt.state}
+        grads = {}
+        hooks = [v.register_post_accumulate_grad_hook(lambda p, k=k: grads.__setitem__(k, p.grad.clone())) for k, v in tr.par.items()]
+        tr.step(it)
+        for h in hooks:
+            h.remove()
+        coef = float(opt.last_norm[1])
+        n, c = O.norm([n64(g) for g in grads.values()], 0.01)
+        assert abs(float(opt.last_norm[0]) - n) <= 2 * E * n and 0 < coef <= 1
+        if bits == 32:
+            for k, v in tr.par.items():
+                m, q = ((n64(state[k][x]) for x in ("exp_avg", "exp_avg_sq")) if k in state else (np.zeros(v.numel()), np.zeros(v.numel())))
+                p1, m1, v1, scale = O.adamw(n64(before[k]), n64(grads[k]), m, q, it, LRS[k], (0.9, 0.999), 1e-15, 0.0, coef)
+                tol = bound32(p1, m1, v1, scale, LRS[k], 0.0, torch.float32)
+                tol = np.where(v1 < 2.0 ** -120, np.maximum(tol, 2 * LRS[k]), tol)          # squares that 32 bits hold as denormals: any update up to its bound
+                assert (np.abs(n64(v) - p1) <= tol).all(), k
+    P = tr.P
+    weights = []
+    for vw in tr.views:
+        act = tr.render(vw)["act"]
+        weights.append(MO().compositing_weights(tr.rasterizer(vw).raster_settings, act["means3D"], act["opacities"], act["scales"], act["rotations"]))
+    weights = torch.stack(weights)
+    scores = torch.zeros(P, device=DEV)
+    kept, scores, extra = opt.evict(scores, 3500, recent=100, weights=weights, extra=[tr.max_radii2D, tr.xyz_gradient_accum, tr.denom])
+    want, _ = O.evict(np.zeros(P, np.float32), 3500, 100, weights.cpu().numpy())
+    assert np.array_equal(kept.cpu().numpy(), want) and scores.shape == (3500,)
+    tr.max_radii2D, tr.xyz_gradient_accum, tr.denom = extra
+    tr.par = {g["name"]: g["params"][0] for g in opt.param_groups}
+    assert tr.P == 3500
+    tr.step(5)
+    opt.append_rows([g["params"][0].detach()[:200] + 0.01 for g in opt.param_groups])
+    tr.par = {g["name"]: g["params"][0] for g in opt.param_groups}
+    tr._reset_stats()
+    for it in range(6, 9):
+        loss = tr.step(it)
+    assert math.isfinite(float(loss)) and all(bool(v.isfinite().all()) for v in tr.par.values())
+    assert float(opt.state[tr.par["xyz"]]["step"][2]) == 8.0
+    if bits == 32:          # the replay's own densification indexes and concatenates "exp_avg" and "exp_avg_sq" itself
+        tr.P1 = 6000
+        tr.densify(4000)
+        tr.step(9)
+        assert opt.state[tr.par["xyz"]]["exp_avg"].shape == (4000, 3)
+        tr.reset_opacity()
+        tr.step(10)
+
+
+def test_c_program_without_python(tmp_path):
+    """nothing here needs Python or torch: the entry points' declarations are C and the library exports them"""
+    import subprocess
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "a.c"
+    src.write_text('#include "gsr.h"\nint main(void){gsr_adamw_args a; gsr_evict_args e; (void)a; (void)e; return gsr_evict_bytes(10) > 0 && gsr_grad_norm_bytes(3) > 0 ? 0 : 1;}\n')
+    lib = os.path.join(root, "gs_localization_amd")
+    subprocess.check_call(["gcc", "-std=c99", "-Wall", "-I" + os.path.join(root, "include"), str(src), "-L" + lib, "-lgsr_hip", "-L/opt/rocm/lib", "-lamdhip64",
+                           "-Wl,-rpath," + lib + ":/opt/rocm/lib", "-o", str(tmp_path / "a")])
+    subprocess.check_call([str(tmp_path / "a")])
