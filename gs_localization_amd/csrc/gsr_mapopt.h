@@ -21,7 +21,7 @@ namespace gsr {
 #define GSR_OPT_WINDOW 256      // elements that share a window of the 8-bit root: four per lane of a wave
 #define GSR_NORM_MAX 160
 
-enum { GSR_T_F32 = 0, GSR_T_BF16 = 1, GSR_T_F16 = 2 };
+enum { GSR_T_F32 = 0, GSR_T_BF16 = 1, GSR_T_F16 = 2, GSR_T_ALIGNED = 256 };          // aligned: opt_load4 may be used
 
 __device__ __forceinline__ float opt_load(const void* p, long long i, int type)
 {
@@ -38,9 +38,38 @@ __device__ __forceinline__ void opt_store(void* p, long long i, int type, float 
     else static_cast<_Float16*>(p)[i] = (_Float16)x;
 }
 
+// Four elements at once, i a multiple of four, the pointer aligned to four of them (16 bytes in 32 bits, 8 in half precision).
+typedef float opt_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t opt_u2 __attribute__((ext_vector_type(2)));
+typedef __bf16 opt_b4 __attribute__((ext_vector_type(4)));
+typedef _Float16 opt_h4 __attribute__((ext_vector_type(4)));
+// STREAM: past the caches (non-temporal), for a launch whose data do not fit the 256 MB behind the L2 anyway: without it the lines
+// that a step leaves there only push out one another.  AdamW over 34.5 M elements (966 MB): 168 us with, 189 without; over 4.6 M (129 MB)
+// 28.6 with, 24.5 without -- the rule is opt_stream() (gsr_mapopt_api.h).
+template <bool STREAM, class T> __device__ __forceinline__ T opt_get(const T* p) { return STREAM ? __builtin_nontemporal_load(p) : *p; }
+template <bool STREAM, class T> __device__ __forceinline__ void opt_put(T* p, T x) { if (STREAM) __builtin_nontemporal_store(x, p); else *p = x; }
+template <int TYPE, bool STREAM>
+__device__ __forceinline__ opt_f4 opt_load4(const void* p, long long i)
+{
+    if (TYPE == GSR_T_F32) return opt_get<STREAM>(reinterpret_cast<const opt_f4*>(static_cast<const float*>(p) + i));
+    const opt_u2 x = opt_get<STREAM>(reinterpret_cast<const opt_u2*>(static_cast<const uint16_t*>(p) + i));
+    if (TYPE == GSR_T_F16) return __builtin_convertvector(__builtin_bit_cast(opt_h4, x), opt_f4);
+    opt_f4 r;
+    r.x = __uint_as_float(x.x << 16); r.y = __uint_as_float(x.x & 0xffff0000u); r.z = __uint_as_float(x.y << 16); r.w = __uint_as_float(x.y & 0xffff0000u);
+    return r;
+}
+template <int TYPE, bool STREAM>
+__device__ __forceinline__ void opt_store4(void* p, long long i, opt_f4 x)
+{
+    if (TYPE == GSR_T_F32) { opt_put<STREAM>(reinterpret_cast<opt_f4*>(static_cast<float*>(p) + i), x); return; }
+    const opt_u2 h = TYPE == GSR_T_F16 ? __builtin_bit_cast(opt_u2, __builtin_convertvector(x, opt_h4)) : __builtin_bit_cast(opt_u2, __builtin_convertvector(x, opt_b4));
+    opt_put<STREAM>(reinterpret_cast<opt_u2*>(static_cast<uint16_t*>(p) + i), h);
+}
+template <int TYPE> __device__ __forceinline__ float opt_load1(const void* p, long long i) { return opt_load(p, i, TYPE); }
+
 // ---- the norm of the gradients --------------------------------------------------------------------------------------------------
 
-struct NormTensor { const void* g; long long n; uint32_t first; int type; };          // first: its first chunk in the launch
+struct NormTensor { const void* g; long long n; uint32_t first; int type; };          // first: its first chunk in the launch; type | GSR_T_ALIGNED
 struct NormArgs {
     int count;
     uint32_t chunks;
@@ -68,18 +97,42 @@ __device__ __forceinline__ double opt_block_sum(double x, double* s)          //
     return threadIdx.x == 0 ? ((s[0] + s[1]) + (s[2] + s[3])) : 0.0;
 }
 
+// A product of two floats is exact in a double: one rounding per element, 2^-53 of the running sum.
+__device__ __forceinline__ void norm_add(double& sum, float x) { sum = __builtin_fma((double)x, (double)x, sum); }
+
+template <int TYPE>
+__device__ __forceinline__ void norm_chunk(const NormTensor& t, long long base, double (&sum)[4])
+{
+    if (t.type & GSR_T_ALIGNED) {
+        opt_f4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const long long i = base + 4 * (u * GSR_OPT_THREADS + (int)threadIdx.x);
+            x[u] = 0.0f;
+            if (i + 4 <= t.n) x[u] = opt_load4<TYPE, false>(t.g, i);
+            else if (i < t.n) { x[u].x = opt_load1<TYPE>(t.g, i); if (i + 1 < t.n) x[u].y = opt_load1<TYPE>(t.g, i + 1); if (i + 2 < t.n) x[u].z = opt_load1<TYPE>(t.g, i + 2); }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) { norm_add(sum[0], x[u].x); norm_add(sum[1], x[u].y); norm_add(sum[2], x[u].z); norm_add(sum[3], x[u].w); }
+    } else {
+        for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < t.n; k += GSR_OPT_THREADS) norm_add(sum[0], opt_load1<TYPE>(t.g, base + k));
+    }
+}
+
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_grad_norm(NormArgs a)
 {
     __shared__ double s[4];
-    double sum = 0.0;          // a product of two floats is exact in a double: one rounding per element, 2^-53 of the running sum
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
     for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
         const NormTensor& t = a.t[opt_find(a.t, a.count, c)];
         const long long base = (long long)(c - t.first) * GSR_OPT_CHUNK;
-        for (int k = threadIdx.x; k < GSR_OPT_CHUNK; k += GSR_OPT_THREADS)
-            if (base + k < t.n) { const double x = opt_load(t.g, base + k, t.type); sum = __builtin_fma(x, x, sum); }
+        const int type = t.type & 15;
+        if (type == GSR_T_F32) norm_chunk<GSR_T_F32>(t, base, sum);
+        else if (type == GSR_T_BF16) norm_chunk<GSR_T_BF16>(t, base, sum);
+        else norm_chunk<GSR_T_F16>(t, base, sum);
     }
-    sum = opt_block_sum(sum, s);
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
+    const double total = opt_block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), s);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
 }
 
 // The partial sums in a fixed order (the result does not depend on which workgroup ran when), then torch.nn.utils.clip_grad_norm_'s
@@ -109,13 +162,12 @@ struct OptTensor {
     const double* lr_device;    // nullable: a rate that a replayed graph reads anew
     double lr, decay;
     long long n;
-    uint32_t first;             // first chunk in the launch
+    uint32_t first;             // its first workgroup in the launch
     uint32_t key;               // 8 bits: seed and place in the list
-    int types;                  // parameter | gradient << 4
+    int types;                  // parameter | gradient << 4 | GSR_T_ALIGNED
 };
 struct OptArgs {
     int count;
-    uint32_t chunks;
     double beta1, beta2;
     float b1, b2, c1, c2, eps;  // (c = 1 - beta)
     float unit, per_unit;       // 8 bits: the ratio's step, and steps per one
@@ -123,59 +175,113 @@ struct OptArgs {
     OptTensor t[GSR_OPT_MAX];
 };
 
-struct OptRates { float shrink, rate, unbias; uint32_t step; };
-__device__ __forceinline__ OptRates opt_rates(const OptArgs& a, const OptTensor& t)
+__device__ __forceinline__ bool opt_aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
+__device__ __forceinline__ float opt_uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(x))); }
+// The step's scalars, formed in 64 bits: by every wave, behind the loads of its first elements (two divisions and a root of 64 bits
+// under their latency), kept in scalar registers.
+//
+// The step counts live on the device, so that a captured graph goes on counting.  They may advance once every workgroup has read them.  A
+// launch of up to GSR_OPT_TICKETS workgroups does it by itself: a workgroup whose waves all have the clock draws a ticket (the fourth
+// word of the launch's first clock, zero between launches), and the one that drew the last advances the clocks when it is done.
+// No fence: nothing but "has read" is handed over (a release at device scope writes the XCD's L2 back, 57 ns per workgroup).  Same-address
+// atomics take turns, 5 ns each whether their workgroup waits or not, so a larger launch leaves it to k_adamw_advance behind it: 34.5 M
+// elements, 8424 workgroups: 302 us with tickets and fences, 209 with tickets, 169 + 4 with the launch.
+#define GSR_OPT_TICKETS 512
+struct OptRates { float shrink, rate, unbias; uint32_t key, ticket; };
+__device__ __forceinline__ void opt_begin(const OptArgs& a, const OptTensor& t, OptRates& r)          // every wave of a workgroup, once
 {
     const double lr = t.lr_device ? *t.lr_device : t.lr;
     const double b1t = t.clock[0] * a.beta1, b2t = t.clock[1] * a.beta2;
-    OptRates r;
-    r.shrink = (float)(1.0 - lr * t.decay);
-    r.rate = (float)((1.0 / (1.0 - b1t)) * lr);
-    r.unbias = (float)(1.0 / sqrt(1.0 - b2t));
-    r.step = (uint32_t)(t.clock[2] + 1.0);
-    return r;
+    r.shrink = opt_uniform((float)(1.0 - lr * t.decay));
+    r.rate = opt_uniform((float)((1.0 / (1.0 - b1t)) * lr));
+    r.unbias = opt_uniform((float)(1.0 / sqrt(1.0 - b2t)));
+    r.key = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t.key + (uint32_t)(t.clock[2] + 1.0)));
+    r.ticket = 0;
+    if (gridDim.x > GSR_OPT_TICKETS) return;
+    __syncthreads();          // all four waves have the clock
+    if (threadIdx.x == 0) r.ticket = __hip_atomic_fetch_add(reinterpret_cast<unsigned*>(a.t[0].clock + 3), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-
-// Every workgroup has read the clocks before it draws a ticket, so the one that draws the last may advance them: the step counts live
-// on the device (a captured graph goes on counting) without a launch of their own.  The ticket is the fourth word of the launch's first
-// clock and is zero between launches.
-__device__ __forceinline__ void opt_advance(const OptArgs& a)
+__device__ __forceinline__ void opt_advance(const OptArgs& a)          // one wave
 {
-    __shared__ int s_last;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = atomicAdd(reinterpret_cast<unsigned*>(a.t[0].clock + 3), 1u) == gridDim.x - 1u;
-    }
-    __syncthreads();
-    if (!s_last) return;
-    for (int i = threadIdx.x; i < a.count; i += GSR_OPT_THREADS) {
+    for (int i = threadIdx.x; i < a.count; i += 64) {
         double* c = a.t[i].clock;
         c[0] *= a.beta1; c[1] *= a.beta2; c[2] += 1.0;
         if (i == 0) c[3] = 0.0;
     }
 }
+__device__ __forceinline__ void opt_end(const OptArgs& a, const OptRates& r)
+{
+    if (gridDim.x <= GSR_OPT_TICKETS && threadIdx.x < 64 && (uint32_t)__builtin_amdgcn_readfirstlane((int)r.ticket) == gridDim.x - 1u) opt_advance(a);
+}
+__global__ void __launch_bounds__(64) k_adamw_advance(OptArgs a) { opt_advance(a); }
 
+__device__ __forceinline__ float adamw_one(const OptArgs& a, const OptRates& r, float coef, float p, float g, float& m, float& v)
+{
+    g *= coef;
+    m = m * a.b1 + g * a.c1;
+    v = v * a.b2 + (g * g) * a.c2;
+    return p * r.shrink - (m / (sqrtf(v) * r.unbias + a.eps)) * r.rate;
+}
+
+template <int PT, int GT, bool STREAM>
+__device__ __forceinline__ void adamw_chunk(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long base)
+{
+    float* pm = static_cast<float*>(t.s0);
+    float* pv = static_cast<float*>(t.s1);
+    opt_f4 p[4], g[4], m[4], v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const long long i = base + 4 * (u * GSR_OPT_THREADS + (int)threadIdx.x);
+        if (i + 4 <= t.n) {
+            p[u] = opt_load4<PT, STREAM>(t.p, i); g[u] = opt_load4<GT, STREAM>(t.g, i);
+            m[u] = opt_load4<GSR_T_F32, STREAM>(pm, i); v[u] = opt_load4<GSR_T_F32, STREAM>(pv, i);
+        }
+    }
+    opt_begin(a, t, r);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const long long i = base + 4 * (u * GSR_OPT_THREADS + (int)threadIdx.x);
+        if (i + 4 <= t.n) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float mm = m[u][k], vv = v[u][k];
+                p[u][k] = adamw_one(a, r, coef, p[u][k], g[u][k], mm, vv);
+                m[u][k] = mm; v[u][k] = vv;
+            }
+            opt_store4<PT, STREAM>(t.p, i, p[u]); opt_store4<GSR_T_F32, STREAM>(pm, i, m[u]); opt_store4<GSR_T_F32, STREAM>(pv, i, v[u]);
+        } else {
+            for (long long j = i; j < t.n; j++) opt_store(t.p, j, PT, adamw_one(a, r, coef, opt_load(t.p, j, PT), opt_load(t.g, j, GT), pm[j], pv[j]));
+        }
+    }
+}
+
+// Pointers that are not aligned to four elements: one element per lane and load, any types.
+__device__ __forceinline__ void adamw_chunk_unaligned(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long base)
+{
+    float* pm = static_cast<float*>(t.s0);
+    float* pv = static_cast<float*>(t.s1);
+    const int pt = t.types & 15, gt = (t.types >> 4) & 15;
+    opt_begin(a, t, r);
+    for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < t.n; k += GSR_OPT_THREADS) {
+        const long long j = base + k;
+        opt_store(t.p, j, pt, adamw_one(a, r, coef, opt_load(t.p, j, pt), opt_load(t.g, j, gt), pm[j], pv[j]));
+    }
+}
+
+template <bool STREAM>
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw(OptArgs a)
 {
     const float coef = a.clip ? a.clip[1] : 1.0f;
-    for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-        const OptTensor& t = a.t[opt_find(a.t, a.count, c)];
-        const OptRates r = opt_rates(a, t);
-        const long long base = (long long)(c - t.first) * GSR_OPT_CHUNK;
-        float* m = static_cast<float*>(t.s0);
-        float* v = static_cast<float*>(t.s1);
-        for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < t.n; k += GSR_OPT_THREADS) {
-            const long long i = base + k;
-            const float g = opt_load(t.g, i, t.types >> 4) * coef;
-            const float m1 = m[i] * a.b1 + g * a.c1;
-            const float v1 = v[i] * a.b2 + (g * g) * a.c2;
-            const float p = opt_load(t.p, i, t.types & 15) * r.shrink - (m1 / (sqrtf(v1) * r.unbias + a.eps)) * r.rate;
-            m[i] = m1; v[i] = v1;
-            opt_store(t.p, i, t.types & 15, p);
-        }
+    const OptTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];          // (of no elements at all: a launch of one workgroup that advances the clocks)
+    OptRates r;
+    const long long base = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK;
+    switch (t.types) {
+#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw_chunk<P, G, STREAM>(a, t, r, coef, base); break;
+    GSR_OPT_CASE(0, 0) GSR_OPT_CASE(0, 1) GSR_OPT_CASE(0, 2) GSR_OPT_CASE(1, 0) GSR_OPT_CASE(1, 1) GSR_OPT_CASE(1, 2) GSR_OPT_CASE(2, 0) GSR_OPT_CASE(2, 1) GSR_OPT_CASE(2, 2)
+#undef GSR_OPT_CASE
+    default: adamw_chunk_unaligned(a, t, r, coef, base);
     }
-    opt_advance(a);
+    opt_end(a, r);
 }
 
 // ---- AdamW with a byte for each moment -------------------------------------------------------------------------------------------
@@ -208,11 +314,12 @@ __device__ __forceinline__ float opt_decode(uint32_t code, uint32_t base)
 {
     return code ? __uint_as_float((code + base) << 19) : 0.0f;
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)          // over 64 lanes, in every lane (DPP, as wave_sum)
 {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)v, off, 64); v = o > v ? o : v; }
-    return v;
+#define GSR_DPP_MAX(ctrl, rm) { const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rm, 0xf, true); v = o > v ? o : v; }
+    GSR_DPP_MAX(0x111, 0xf) GSR_DPP_MAX(0x112, 0xf) GSR_DPP_MAX(0x114, 0xf) GSR_DPP_MAX(0x118, 0xf) GSR_DPP_MAX(0x142, 0xa) GSR_DPP_MAX(0x143, 0xc)
+#undef GSR_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ uint32_t opt_window(uint32_t largest)          // of the block's largest finite root, by its bits
 {
@@ -220,77 +327,186 @@ __device__ __forceinline__ uint32_t opt_window(uint32_t largest)          // of 
     return w > 0 ? (uint32_t)w : 0u;
 }
 
+// sqrt of four values >= 0 (or infinite, or NaN), correctly rounded.  The instruction is within one ulp; s - ulp is nearer exactly if
+// x <= s (s - ulp) (the midpoint's square is that plus ulp^2 / 4), s + ulp exactly if x > s (s + ulp).  sqrtf spends five more
+// instructions on scaling arguments whose residual could underflow: here one test per wave sends those to it.
+__device__ __forceinline__ void opt_sqrt4(const float (&x)[4], float (&s)[4])
+{
+    uint32_t least = __float_as_uint(x[0]) - 1u;          // (0 wraps to the largest: it needs no scaling)
+#pragma unroll
+    for (int k = 1; k < 4; k++) { const uint32_t b = __float_as_uint(x[k]) - 1u; least = b < least ? b : least; }
+    if (__any(least < 0x0f800000u)) {          // something in (0, 2^-96]
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] = sqrtf(x[k]);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float y = __builtin_amdgcn_sqrtf(x[k]);
+        const float lo = __uint_as_float(__float_as_uint(y) - 1u), hi = __uint_as_float(__float_as_uint(y) + 1u);
+        const float rl = __builtin_fmaf(-lo, y, x[k]), rh = __builtin_fmaf(-hi, y, x[k]);          // (at 0, infinity and NaN: NaN or 0, y stays)
+        s[k] = rh > 0.0f ? hi : (rl <= 0.0f ? lo : y);
+    }
+}
+
+// One wave, four blocks of 256 from `start`, all loads in flight together (two of them: 143 us for 132 over 47 M elements): four consecutive elements per lane.  FULL: every block lies inside the tensor and all
+// pointers are aligned (PT, GT: the types); otherwise element by element, any types.
+template <int PT, int GT, bool FULL, bool STREAM>
+__device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long start)
+{
+    const int pt = FULL ? PT : t.types & 15, gt = FULL ? GT : (t.types >> 4) & 15;
+    const int lane = threadIdx.x & 63;
+    uint8_t* rms = static_cast<uint8_t*>(t.s0);
+    int8_t* ratio = static_cast<int8_t*>(t.s1);
+    opt_f4 p[4], g[4];
+    uint32_t cu[4], cr[4], old[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const long long s = start + b * GSR_OPT_WINDOW, i = s + 4 * lane;
+        p[b] = 0.0f; g[b] = 0.0f; cu[b] = cr[b] = old[b] = 0u;
+        if (FULL) {
+            p[b] = opt_load4<PT, STREAM>(t.p, i); g[b] = opt_load4<GT, STREAM>(t.g, i);
+            cu[b] = opt_get<STREAM>(reinterpret_cast<const uint32_t*>(rms + i)); cr[b] = opt_get<STREAM>(reinterpret_cast<const uint32_t*>(ratio + i));
+            old[b] = t.window[s / GSR_OPT_WINDOW];
+        } else if (s < t.n) {
+            old[b] = t.window[s / GSR_OPT_WINDOW];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k < t.n) {
+                    p[b][k] = opt_load(t.p, i + k, pt); g[b][k] = opt_load(t.g, i + k, gt);
+                    cu[b] |= (uint32_t)rms[i + k] << (8 * k); cr[b] |= (uint32_t)(uint8_t)ratio[i + k] << (8 * k);
+                }
+        }
+    }
+    opt_begin(a, t, r);
+    const uint32_t key = opt_mix(r.key);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const long long s = start + b * GSR_OPT_WINDOW, i = s + 4 * lane;
+        if (!FULL && s >= t.n) break;          // (the whole wave)
+        const uint32_t was = 16u * old[b] + 1u;
+        float m1[4], v1[4], u1[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float u = opt_decode((cu[b] >> (8 * k)) & 255u, was);
+            const float x = g[b][k] * coef;
+            m1[k] = (((float)(int8_t)(cr[b] >> (8 * k)) * a.unit) * u) * a.b1 + x * a.c1;
+            v1[k] = (u * u) * a.b2 + (x * x) * a.c2;
+        }
+        opt_sqrt4(v1, u1);
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            p[b][k] = p[b][k] * r.shrink - (m1[k] / (u1[k] * r.unbias + a.eps)) * r.rate;
+            top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
+        }
+        top = wave_max_u32(top);
+        if (top >= 0x7f800000u) {          // an infinite root or a NaN (the whole wave comes here, or none): its neighbours' window is that of the finite ones
+            top = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (__float_as_uint(u1[k]) >= 0x7f800000u) u1[k] = __builtin_inff();          // -> code 255
+                else top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
+                if (m1[k] != m1[k]) m1[k] = 0.0f;
+            }
+            top = wave_max_u32(top);
+        }
+        const uint32_t w = opt_window(top), now = 16u * w + 1u;
+        // (the upper half of the quad's number is the whole block's)
+        const uint32_t h = opt_mix(((((uint32_t)(s >> 2) + lane) * 0x9E3779B1u) ^ key) + (uint32_t)(s >> 34) * 0x85EBCA77u);
+        uint32_t nu = 0, nr = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t d = opt_dither(h, k), bits = __float_as_uint(u1[k]);
+            int code = (int)((bits + (d >> 13)) >> 19) - (int)now;
+            code = code < 1 ? 1 : (code > 255 ? 255 : code);
+            code = bits == 0u ? 0 : code;
+            const float u = __uint_as_float(((uint32_t)code + now) << 19);          // (of a code 0: some number > 0, the quotient is not used)
+            const float q = floorf((m1[k] / u) * a.per_unit + (float)(d & 8191u) * (1.0f / 8192.0f));
+            const int n = bits == 0u ? 0 : (int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f);
+            nu |= (uint32_t)code << (8 * k);
+            nr |= ((uint32_t)n & 255u) << (8 * k);
+        }
+        if (FULL) {
+            opt_store4<PT, STREAM>(t.p, i, p[b]);
+            opt_put<STREAM>(reinterpret_cast<uint32_t*>(rms + i), nu); opt_put<STREAM>(reinterpret_cast<uint32_t*>(ratio + i), nr);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k < t.n) { opt_store(t.p, i + k, pt, p[b][k]); rms[i + k] = (uint8_t)(nu >> (8 * k)); ratio[i + k] = (int8_t)(nr >> (8 * k)); }
+        }
+        if (lane == 0) t.window[s / GSR_OPT_WINDOW] = (uint8_t)w;
+    }
+}
+
+template <bool STREAM>
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw8(OptArgs a)
 {
     const float coef = a.clip ? a.clip[1] : 1.0f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-        const OptTensor& t = a.t[opt_find(a.t, a.count, c)];
-        const OptRates r = opt_rates(a, t);
-        const uint32_t key = opt_mix(t.key + r.step);
-        uint8_t* rms = static_cast<uint8_t*>(t.s0);
-        int8_t* ratio = static_cast<int8_t*>(t.s1);
-        for (int b = wave; b < GSR_OPT_CHUNK / GSR_OPT_WINDOW; b += 4) {
-            const long long start = (long long)(c - t.first) * GSR_OPT_CHUNK + b * GSR_OPT_WINDOW;
-            if (start >= t.n) break;          // (the whole wave)
-            const long long i0 = start + 4 * lane;
-            const uint32_t old = 16u * t.window[start / GSR_OPT_WINDOW] + 1u;
-            float m1[4], u1[4];
-            uint32_t top = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                m1[k] = u1[k] = 0.0f;
-                if (i0 + k < t.n) {
-                    const float u = opt_decode(rms[i0 + k], old);
-                    const float g = opt_load(t.g, i0 + k, t.types >> 4) * coef;
-                    m1[k] = (((float)ratio[i0 + k] * a.unit) * u) * a.b1 + g * a.c1;
-                    u1[k] = sqrtf((u * u) * a.b2 + (g * g) * a.c2);
-                    const float p = opt_load(t.p, i0 + k, t.types & 15) * r.shrink - (m1[k] / (u1[k] * r.unbias + a.eps)) * r.rate;
-                    opt_store(t.p, i0 + k, t.types & 15, p);
-                    const uint32_t bits = __float_as_uint(u1[k]) & 0x7fffffffu;
-                    if (bits < 0x7f800000u && bits > top) top = bits;          // (an infinite root or a NaN leaves its neighbours' window alone)
-                }
-            }
-            const uint32_t w = opt_window(wave_max_u32(top)), now = 16u * w + 1u;
-            const uint32_t j = (uint32_t)(i0 >> 2), jh = (uint32_t)(i0 >> 34);
-            const uint32_t h = opt_mix(((j * 0x9E3779B1u) ^ key) + jh * 0x85EBCA77u);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (i0 + k >= t.n) break;
-                const uint32_t d = opt_dither(h, k);
-                const uint32_t bits = __float_as_uint(u1[k]) & 0x7fffffffu;
-                int code = (int)((bits + (d >> 13)) >> 19) - (int)now;
-                code = code < 1 ? 1 : (code > 255 ? 255 : code);
-                if (bits >= 0x7f800000u) code = 255;
-                if (bits == 0u) code = 0;
-                const float u = opt_decode((uint32_t)code, now);
-                float q = floorf((m1[k] / u) * a.per_unit + (float)(d & 8191u) * (1.0f / 8192.0f));
-                q = q < -127.0f ? -127.0f : (q > 127.0f ? 127.0f : q);
-                if (!(u > 0.0f) || q != q) q = 0.0f;
-                rms[i0 + k] = (uint8_t)code;
-                ratio[i0 + k] = (int8_t)q;
-            }
-            if (lane == 0) t.window[start / GSR_OPT_WINDOW] = (uint8_t)w;
+    const OptTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];
+    OptRates r;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const long long start = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK + wave * (GSR_OPT_CHUNK / 4);
+    if (start < t.n) {
+        switch (start + GSR_OPT_CHUNK / 4 <= t.n ? t.types : 0) {
+#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw8_blocks<P, G, true, STREAM>(a, t, r, coef, start); break;
+        GSR_OPT_CASE(0, 0) GSR_OPT_CASE(0, 1) GSR_OPT_CASE(0, 2) GSR_OPT_CASE(1, 0) GSR_OPT_CASE(1, 1) GSR_OPT_CASE(1, 2) GSR_OPT_CASE(2, 0) GSR_OPT_CASE(2, 1) GSR_OPT_CASE(2, 2)
+#undef GSR_OPT_CASE
+        default: adamw8_blocks<0, 0, false, false>(a, t, r, coef, start);
         }
+    } else {
+        opt_begin(a, t, r);          // (to the other waves' barrier)
     }
-    opt_advance(a);
+    opt_end(a, r);
 }
 
-struct MomentTensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg; void* root; long long n; uint32_t first; };
-struct MomentArgs { int count; uint32_t chunks; float unit; int type; MomentTensor t[GSR_OPT_MAX]; };
+struct MomentTensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg; void* root; long long n; uint32_t first; int aligned; };
+struct MomentArgs { int count; float unit; int type; MomentTensor t[GSR_OPT_MAX]; };
 
-__global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
+template <int TYPE>
+__device__ __forceinline__ void moments_chunk(const MomentArgs& a, const MomentTensor& t, long long base)
 {
-    for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-        const MomentTensor& t = a.t[opt_find(a.t, a.count, c)];
-        const long long base = (long long)(c - t.first) * GSR_OPT_CHUNK;
+    if (t.aligned) {
+        uint32_t cu[4], cr[4], w[4];
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const long long i = base + 4 * (v * GSR_OPT_THREADS + (int)threadIdx.x);
+            cu[v] = cr[v] = w[v] = 0u;
+            if (i < t.n) w[v] = t.window[i / GSR_OPT_WINDOW];
+            if (i + 4 <= t.n) { cu[v] = *reinterpret_cast<const uint32_t*>(t.rms + i); cr[v] = *reinterpret_cast<const uint32_t*>(t.ratio + i); }
+            else for (int k = 0; i + k < t.n; k++) { cu[v] |= (uint32_t)t.rms[i + k] << (8 * k); cr[v] |= (uint32_t)(uint8_t)t.ratio[i + k] << (8 * k); }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const long long i = base + 4 * (v * GSR_OPT_THREADS + (int)threadIdx.x);
+            opt_f4 m, u;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                u[k] = opt_decode((cu[v] >> (8 * k)) & 255u, 16u * w[v] + 1u);
+                m[k] = ((float)(int8_t)(cr[v] >> (8 * k)) * a.unit) * u[k];
+            }
+            if (i + 4 <= t.n) { opt_store4<TYPE, false>(t.exp_avg, i, m); opt_store4<TYPE, false>(t.root, i, u); }
+            else
+#pragma unroll
+                for (int k = 0; k < 4; k++) if (i + k < t.n) { opt_store(t.exp_avg, i + k, TYPE, m[k]); opt_store(t.root, i + k, TYPE, u[k]); }
+        }
+    } else {
         for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < t.n; k += GSR_OPT_THREADS) {
             const long long i = base + k;
             const float u = opt_decode(t.rms[i], 16u * t.window[i / GSR_OPT_WINDOW] + 1u);
-            opt_store(t.exp_avg, i, a.type, ((float)t.ratio[i] * a.unit) * u);
-            opt_store(t.root, i, a.type, u);
+            opt_store(t.exp_avg, i, TYPE, ((float)t.ratio[i] * a.unit) * u);
+            opt_store(t.root, i, TYPE, u);
         }
     }
+}
+
+__global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
+{
+    const MomentTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];
+    const long long base = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK;
+    if (a.type == GSR_T_F32) moments_chunk<GSR_T_F32>(a, t, base);
+    else if (a.type == GSR_T_BF16) moments_chunk<GSR_T_BF16>(a, t, base);
+    else moments_chunk<GSR_T_F16>(a, t, base);
 }
 
 // ---- eviction by accumulated compositing weight ----------------------------------------------------------------------------------
@@ -298,10 +514,16 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
 // A pixel reads the map as a query reads a cache: splat i with the weight alpha_i T_i.  The rows that stay are the `recent` newest (no
 // view has weighed them yet) and, of the others, the k with the largest accumulated weight; ties go to the lowest index, NaN counts as -inf.
 // The k-th largest is found exactly by a radix select on order-preserving bit patterns (11 + 11 + 10 bits, one histogram launch each),
-// the rows' places by counting per tile of rows; every tensor of the map and of its optimiser is then compacted in one launch.
+// the rows' places by counting per tile of rows; every tensor of the map and of its optimiser is then compacted in one launch.  No
+// workgroup ever waits for another: a launch's end is the only barrier between them.
 
+#define GSR_EV_UNITS 16         // units of a lane whose loads are in flight together (4: 178 us for 1.35 M rows of 281 bytes, 8: 173, 16: 154)
+#define GSR_EV_BLOCKS 4         // blocks of codes likewise
 #define GSR_EV_BINS 2048
-#define GSR_EV_TILES 1024       // tiles of rows: few enough for every workgroup to add up its predecessors' counts by itself
+#define GSR_EV_COPIES 8         // of the first histogram in LDS: its bins are exponents, a wave's lanes meet in few of them
+#define GSR_EV_TILE 1024        // rows of a tile, or a multiple of it
+#define GSR_EV_TILES 2048       // tiles at most: every workgroup adds up its predecessors' counts by itself
+#define GSR_EV_SMALL 8192       // rows up to which one workgroup does it all
 
 struct EvictArgs {
     int P, views, old, k;       // old = P - recent: the rows that compete; k of them stay
@@ -309,24 +531,57 @@ struct EvictArgs {
     const float* scores; const float* weights;
     float* total;               // [P] accumulated weights
     uint32_t* hist;             // [3][GSR_EV_BINS]
+    uint32_t* found;            // [3][2]: leading bits of the k-th largest key and its rank among those that share them, by level
     uint2* counts;              // [tiles] (above, equal)
-    int tiles, tile_rows;
+    int tile_rows;
     long long* kept; float* scores_out;
 };
 
+// The accumulated weights of U rows, summed in the views' order.  No load waits for another: rows behind the end load the last row again,
+// views behind the last the last view (a load under a condition is waited for where it stands: k_evict_scores 22 us at 1.5 M rows and 4 views, 15 so).
+template <int U>
+__device__ __forceinline__ void evict_scores(const EvictArgs& a, const long long (&i)[U], float (&s)[U])
+{
+    long long j[U];
+    float x[U];
+    double w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) { j[u] = i[u] < a.P ? i[u] : a.P - 1; x[u] = a.scores[j[u]]; w[u] = 0.0; }
+    for (int v = 0; v < a.views; v += 4) {
+        float y[4][U];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int u = 0; u < U; u++) y[k][u] = a.weights[(long long)(v + k < a.views ? v + k : a.views - 1) * a.P + j[u]];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (v + k < a.views) {
+#pragma unroll
+                for (int u = 0; u < U; u++) w[u] += (double)y[k][u];
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) s[u] = (float)((double)x[u] * a.decay + w[u]);
+}
 __device__ __forceinline__ uint32_t evict_key(float x)          // larger score <=> larger key; NaN as -inf, -0 as +0
 {
     if (x != x) x = -__builtin_inff();
     const uint32_t b = __float_as_uint(x + 0.0f);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
+// No key is 0 or 2^32 - 1 (-inf has 0x007fffff, +inf 0xff800000).
+#define GSR_EV_NONE 0xffffffffu
+#define GSR_EV_ALL 0u
 
-// Which bin, counted from the highest, holds the k-th largest (k >= 1), and its rank among that bin's.  256 threads, nb = 256 * per.
-__device__ __forceinline__ void evict_pick(const uint32_t* __restrict__ hist, int per, uint32_t k, uint32_t* s_tmp /*[8]*/, uint32_t& bin, uint32_t& k_rem)
+// Which bin, counted from the highest, holds the k-th largest (k >= 1), and its rank among that bin's.  T threads, all of them; NB bins.
+template <int T, int NB>
+__device__ __forceinline__ void evict_pick(const uint32_t* hist, uint32_t k, uint32_t* s_tmp /*[T / 64 + 2]*/, uint32_t& bin, uint32_t& rank)
 {
-    const int t = threadIdx.x, nb = 256 * per;
-    uint32_t c[8], sum = 0;
-    for (int j = 0; j < per; j++) { c[j] = hist[nb - 1 - (t * per + j)]; sum += c[j]; }
+    constexpr int per = NB / T;
+    const int t = threadIdx.x;
+    uint32_t c[per], sum = 0;
+#pragma unroll
+    for (int j = 0; j < per; j++) { c[j] = hist[NB - 1 - (t * per + j)]; sum += c[j]; }
     uint32_t incl = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -339,196 +594,338 @@ __device__ __forceinline__ void evict_pick(const uint32_t* __restrict__ hist, in
     for (int w = 0; w < (t >> 6); w++) incl += s_tmp[w];
     uint32_t before = incl - sum;
     if (k > before && k <= incl) {
-        int j = 0;
-        while (j < per - 1 && k > before + c[j]) { before += c[j]; j++; }
-        s_tmp[4] = (uint32_t)(nb - 1 - (t * per + j));
-        s_tmp[5] = k - before;
+#pragma unroll
+        for (int j = 0; j < per; j++) {
+            if (k > before && k <= before + c[j]) { s_tmp[T / 64] = (uint32_t)(NB - 1 - (t * per + j)); s_tmp[T / 64 + 1] = k - before; }
+            before += c[j];
+        }
     }
     __syncthreads();
-    bin = s_tmp[4];
-    k_rem = s_tmp[5];
+    bin = s_tmp[T / 64];
+    rank = s_tmp[T / 64 + 1];
 }
 
-__device__ __forceinline__ void evict_flush(const uint32_t* s_hist, uint32_t* __restrict__ hist, int nb)
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v)          // over 64 lanes, in every lane (DPP)
 {
-    __syncthreads();
-    for (int b = threadIdx.x; b < nb; b += 256)
-        if (s_hist[b]) atomicAdd(&hist[b], s_hist[b]);
+#define GSR_DPP_SUM(ctrl, rm) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rm, 0xf, true);
+    GSR_DPP_SUM(0x111, 0xf) GSR_DPP_SUM(0x112, 0xf) GSR_DPP_SUM(0x114, 0xf) GSR_DPP_SUM(0x118, 0xf) GSR_DPP_SUM(0x142, 0xa) GSR_DPP_SUM(0x143, 0xc)
+#undef GSR_DPP_SUM
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-__global__ void __launch_bounds__(256) k_evict_scores(EvictArgs a)
+// Launch 1: the accumulated weights and the histogram of their keys' upper 11 bits.
+__global__ void __launch_bounds__(512) k_evict_scores(EvictArgs a)
 {
-    __shared__ uint32_t s_hist[GSR_EV_BINS];
-    for (int b = threadIdx.x; b < GSR_EV_BINS; b += 256) s_hist[b] = 0u;
+    __shared__ uint32_t s_hist[GSR_EV_COPIES * (GSR_EV_BINS + 1)];          // (a bin's copies in banks of their own)
+    for (int b = threadIdx.x; b < GSR_EV_COPIES * (GSR_EV_BINS + 1); b += 512) s_hist[b] = 0u;
     __syncthreads();
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.P; i += (long long)gridDim.x * 256) {
-        double x = (double)a.scores[i] * a.decay;
-        double w = 0.0;
-        for (int v = 0; v < a.views; v++) w += (double)a.weights[(long long)v * a.P + i];
-        const float s = (float)(x + w);
-        a.total[i] = s;
-        if (i < a.old) atomicAdd(&s_hist[evict_key(s) >> 21], 1u);
+    uint32_t* const own = s_hist + (threadIdx.x & (GSR_EV_COPIES - 1)) * (GSR_EV_BINS + 1);
+    const long long step = (long long)gridDim.x * 2048;
+    for (long long i0 = (long long)blockIdx.x * 2048 + threadIdx.x; i0 < a.P; i0 += step) {
+        const long long i[4] = {i0, i0 + 512, i0 + 1024, i0 + 1536};
+        float s[4];
+        evict_scores(a, i, s);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (i[u] < a.P) a.total[i[u]] = s[u];
+            if (i[u] < a.old) atomicAdd(&own[evict_key(s[u]) >> 21], 1u);
+        }
     }
-    evict_flush(s_hist, a.hist, GSR_EV_BINS);
+    __syncthreads();
+    for (int b = threadIdx.x; b < GSR_EV_BINS; b += 512) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int c = 0; c < GSR_EV_COPIES; c++) n += s_hist[c * (GSR_EV_BINS + 1) + b];
+        if (n) atomicAdd(&a.hist[b], n);
+    }
 }
 
+// Launches 2 and 3: the histogram of the next bits among the keys that share the k-th largest's leading ones.  Few, large workgroups:
+// each flushes up to 2048 bins with global atomics (1024 workgroups of 256: 18 us at 1.5 M rows).
 template <int LEVEL>
-__global__ void __launch_bounds__(256) k_evict_hist(EvictArgs a)
+__global__ void __launch_bounds__(1024) k_evict_hist(EvictArgs a)
 {
     __shared__ uint32_t s_hist[GSR_EV_BINS];
-    __shared__ uint32_t s_tmp[8];
+    __shared__ uint32_t s_tmp[1024 / 64 + 2];
     constexpr int NB = LEVEL == 2 ? GSR_EV_BINS : GSR_EV_BINS / 2;
-    for (int b = threadIdx.x; b < NB; b += 256) s_hist[b] = 0u;
-    uint32_t prefix, k;
-    evict_pick(a.hist, GSR_EV_BINS / 256, (uint32_t)a.k, s_tmp, prefix, k);
-    if (LEVEL == 3) {
+    for (int b = threadIdx.x; b < NB; b += 1024) s_hist[b] = 0u;
+    uint32_t prefix, rank;
+    if (LEVEL == 2) evict_pick<1024, GSR_EV_BINS>(a.hist, (uint32_t)a.k, s_tmp, prefix, rank);
+    else {
         uint32_t bin;
-        evict_pick(a.hist + GSR_EV_BINS, GSR_EV_BINS / 256, k, s_tmp, bin, k);
-        prefix = (prefix << 11) | bin;
+        evict_pick<1024, GSR_EV_BINS>(a.hist + GSR_EV_BINS, a.found[1], s_tmp, bin, rank);
+        prefix = (a.found[0] << 11) | bin;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) { a.found[2 * (LEVEL - 2)] = prefix; a.found[2 * (LEVEL - 2) + 1] = rank; }
+    const long long step = (long long)gridDim.x * 8192;
+    for (long long i0 = (long long)blockIdx.x * 8192 + threadIdx.x; i0 < a.old; i0 += step) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) x[u] = a.total[i0 + 1024 * u < a.old ? i0 + 1024 * u : a.old - 1];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const uint32_t key = evict_key(x[u]);
+            if (i0 + 1024 * u >= a.old) break;
+            if (LEVEL == 2) { if ((key >> 21) == prefix) atomicAdd(&s_hist[(key >> 10) & 2047u], 1u); }
+            else            { if ((key >> 10) == prefix) atomicAdd(&s_hist[key & 1023u], 1u); }
+        }
     }
     __syncthreads();
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.old; i += (long long)gridDim.x * 256) {
-        const uint32_t key = evict_key(a.total[i]);
-        if (LEVEL == 2) { if ((key >> 21) == prefix) atomicAdd(&s_hist[(key >> 10) & 2047u], 1u); }
-        else            { if ((key >> 10) == prefix) atomicAdd(&s_hist[key & 1023u], 1u); }
-    }
-    evict_flush(s_hist, a.hist + (LEVEL - 1) * GSR_EV_BINS, NB);
+    for (int b = threadIdx.x; b < NB; b += 1024)
+        if (s_hist[b]) atomicAdd(&a.hist[(LEVEL - 1) * GSR_EV_BINS + b], s_hist[b]);
 }
 
-// The smallest key that stays, and how many rows with exactly that key do.
-__device__ __forceinline__ void evict_threshold(const EvictArgs& a, uint32_t* s_tmp, uint32_t& key, uint32_t& ties)
-{
-    if (a.k == 0) { key = 0xffffffffu; ties = 0u; return; }                    // (no row has that key: +inf has 0xff800000)
-    if (a.k == a.old) { key = 0u; ties = 0u; return; }                         // (nor this one: -inf has 0x007fffff)
-    uint32_t b1, b2, b3, k;
-    evict_pick(a.hist, GSR_EV_BINS / 256, (uint32_t)a.k, s_tmp, b1, k);
-    evict_pick(a.hist + GSR_EV_BINS, GSR_EV_BINS / 256, k, s_tmp, b2, k);
-    evict_pick(a.hist + 2 * GSR_EV_BINS, GSR_EV_BINS / 512, k, s_tmp, b3, ties);
-    key = (b1 << 21) | (b2 << 10) | b3;
-}
-
+// Launch 4: the smallest key that stays and how many rows with exactly that key do; how many of either kind each tile has.
 __global__ void __launch_bounds__(256) k_evict_count(EvictArgs a)
 {
-    __shared__ uint32_t s_tmp[8];
+    __shared__ uint32_t s_tmp[256 / 64 + 2];
     __shared__ uint32_t s_n[2];
-    uint32_t key, ties;
-    evict_threshold(a, s_tmp, key, ties);
+    uint32_t key, ties = 0u;
+    if (a.k == 0) key = GSR_EV_NONE;
+    else if (a.k == a.old) key = GSR_EV_ALL;
+    else {
+        evict_pick<256, GSR_EV_BINS / 2>(a.hist + 2 * GSR_EV_BINS, a.found[3], s_tmp, key, ties);
+        key |= a.found[2] << 10;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) { a.found[4] = key; a.found[5] = ties; }
     if (threadIdx.x < 2) s_n[threadIdx.x] = 0u;
     __syncthreads();
     uint32_t above = 0, equal = 0;
     const long long lo = (long long)blockIdx.x * a.tile_rows;
-    for (int r = threadIdx.x; r < a.tile_rows && lo + r < a.old; r += 256) {
-        const uint32_t x = evict_key(a.total[lo + r]);
-        above += x > key; equal += x == key;
+    for (int r0 = 0; r0 < a.tile_rows; r0 += 1024) {
+        float x[4];
+        if (r0 + 1024 <= a.tile_rows && lo + r0 + 1024 <= a.old) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = a.total[lo + r0 + 256 * u + threadIdx.x];
+#pragma unroll
+            for (int u = 0; u < 4; u++) { above += evict_key(x[u]) > key; equal += evict_key(x[u]) == key; }
+        } else {
+            for (int r = r0 + (int)threadIdx.x; r < a.tile_rows && lo + r < a.old && r < r0 + 1024; r += 256) { const uint32_t k = evict_key(a.total[lo + r]); above += k > key; equal += k == key; }
+        }
     }
-    atomicAdd(&s_n[0], above); atomicAdd(&s_n[1], equal);
+    above = wave_sum_u32(above); equal = wave_sum_u32(equal);
+    if ((threadIdx.x & 63) == 0) { atomicAdd(&s_n[0], above); atomicAdd(&s_n[1], equal); }
     __syncthreads();
     if (threadIdx.x == 0) a.counts[blockIdx.x] = make_uint2(s_n[0], s_n[1]);
 }
 
+// The rows of one pass that stay, written in order: thread t has rows lo + T u + t, u < U; `above`, `equal`: how many were counted before `lo`,
+// advanced.  Two barriers; s_n [U * T / 64].
+template <int T, int U>
+__device__ __forceinline__ void evict_emit_pass(const EvictArgs& a, long long lo, const float (&s)[U], int rows, uint32_t key, uint32_t ties,
+                                                uint2* s_n, uint32_t& above, uint32_t& equal)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    unsigned long long ma[U], me[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int r = T * u + t;
+        const bool in = r < rows && lo + r < a.old;
+        const uint32_t x = evict_key(s[u]);
+        ma[u] = __ballot(in && x > key); me[u] = __ballot(in && x == key);
+        if (lane == 0) s_n[u * (T / 64) + wave] = make_uint2((uint32_t)__popcll(ma[u]), (uint32_t)__popcll(me[u]));
+    }
+    __syncthreads();
+    const unsigned long long below = (1ull << lane) - 1ull;
+    uint32_t na = above, ne = equal;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) {
+            if (w == wave) {
+                const int r = T * u + t;
+                const long long i = lo + r;
+                const uint32_t ia = na + (uint32_t)__popcll(ma[u] & below), ie = ne + (uint32_t)__popcll(me[u] & below);
+                long long at = -1;
+                if (r < rows && i >= a.old) at = (long long)a.k + (i - a.old);
+                else if ((ma[u] >> lane) & 1ull || ((me[u] >> lane) & 1ull && ie < ties)) at = (long long)ia + (ie < ties ? ie : ties);
+                if (at >= 0) { a.kept[at] = i; a.scores_out[at] = s[u]; }
+            }
+            const uint2 n = s_n[u * (T / 64) + w];
+            na += n.x; ne += n.y;
+        }
+    }
+    above = na; equal = ne;
+    __syncthreads();
+}
+
+// Launch 5: the rows that stay, in their order.
 __global__ void __launch_bounds__(256) k_evict_emit(EvictArgs a)
 {
-    __shared__ uint32_t s_tmp[8];
-    __shared__ uint32_t s_wave[4][2];
+    __shared__ uint2 s_n[16];
     __shared__ uint32_t s_base[2];
-    uint32_t key, ties;
-    evict_threshold(a, s_tmp, key, ties);
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x;
+    const long long lo = (long long)blockIdx.x * a.tile_rows;
+    const int rows = (int)(a.P - lo < a.tile_rows ? a.P - lo : a.tile_rows);
+    float s[4];
+    const auto read = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) s[u] = a.total[lo + (r0 + 256 * u + t < rows ? r0 + 256 * u + t : 0)];
+    };
+    read(0);
     if (t < 2) s_base[t] = 0u;
     __syncthreads();
     uint32_t above = 0, equal = 0;          // of the tiles in front
-    for (int b = t; b < (int)blockIdx.x; b += 256) { const uint2 n = a.counts[b]; above += n.x; equal += n.y; }
-    atomicAdd(&s_base[0], above); atomicAdd(&s_base[1], equal);
+    {
+        uint2 n[GSR_EV_TILES / 256];
+#pragma unroll
+        for (int j = 0; j < GSR_EV_TILES / 256; j++) n[j] = a.counts[256 * j + t < (int)blockIdx.x ? 256 * j + t : 0];
+#pragma unroll
+        for (int j = 0; j < GSR_EV_TILES / 256; j++) if (256 * j + t < (int)blockIdx.x) { above += n[j].x; equal += n[j].y; }
+    }
+    above = wave_sum_u32(above); equal = wave_sum_u32(equal);
+    if ((t & 63) == 0) { atomicAdd(&s_base[0], above); atomicAdd(&s_base[1], equal); }
+    const uint32_t key = a.found[4], ties = a.found[5];
     __syncthreads();
     above = s_base[0]; equal = s_base[1];
-    const long long lo = (long long)blockIdx.x * a.tile_rows;
-    for (int r0 = 0; r0 < a.tile_rows; r0 += 256) {          // (uniform: every thread meets the barriers)
-        const long long i = lo + r0 + t;
-        const bool in = r0 + t < a.tile_rows && i < a.P, recent = in && i >= a.old;
-        const float s = in ? a.total[i] : 0.0f;
-        const uint32_t x = in && !recent ? evict_key(s) : 0u;
-        const bool is_above = in && !recent && x > key, is_equal = in && !recent && x == key;
-        const unsigned long long ma = __ballot(is_above), me = __ballot(is_equal), below = (1ull << lane) - 1ull;
-        if (lane == 0) { s_wave[wave][0] = (uint32_t)__popcll(ma); s_wave[wave][1] = (uint32_t)__popcll(me); }
-        __syncthreads();
-        uint32_t na = above, ne = equal, ta = 0, te = 0;
-        for (int w = 0; w < 4; w++) {
-            if (w < wave) { na += s_wave[w][0]; ne += s_wave[w][1]; }
-            ta += s_wave[w][0]; te += s_wave[w][1];
-        }
-        na += (uint32_t)__popcll(ma & below); ne += (uint32_t)__popcll(me & below);
-        long long at = -1;
-        if (recent) at = (long long)a.k + (i - a.old);
-        else if (is_above || (is_equal && ne < ties)) at = (long long)na + (ne < ties ? ne : ties);
-        if (at >= 0) { a.kept[at] = i; a.scores_out[at] = s; }
-        above += ta; equal += te;
-        __syncthreads();
+    for (int r0 = 0; r0 < rows; r0 += GSR_EV_TILE) {
+        if (r0) read(r0);
+        evict_emit_pass<256, 4>(a, lo + r0, s, rows - r0, key, ties, s_n, above, equal);
     }
+}
+
+// All of it for a small map: scores in registers, histograms in LDS.
+__global__ void __launch_bounds__(1024) k_evict_small(EvictArgs a)
+{
+    constexpr int U = GSR_EV_SMALL / 1024;
+    __shared__ uint32_t s_hist[GSR_EV_BINS];
+    __shared__ uint32_t s_tmp[1024 / 64 + 2];
+    __shared__ uint2 s_n[16 * U];
+    const int t = threadIdx.x;
+    long long i[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) i[u] = 1024 * u + t;
+    evict_scores(a, i, s);
+    uint32_t key = GSR_EV_NONE, ties = 0u;
+    if (a.k > 0 && a.k == a.old) key = GSR_EV_ALL;
+    else if (a.k > 0) {
+        uint32_t prefix = 0u, rank = (uint32_t)a.k, bin;
+#pragma unroll 1
+        for (int level = 0; level < 3; level++) {          // 11, 11 and 10 bits (the last histogram's upper half stays empty)
+            const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, known = level == 0 ? 0 : level == 1 ? 21 : 10;
+            __syncthreads();
+            s_hist[t] = 0u; s_hist[1024 + t] = 0u;
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t x = evict_key(s[u]);
+                if (1024 * u + t < a.old && (level == 0 || (x >> known) == prefix)) atomicAdd(&s_hist[(x >> shift) & (level == 2 ? 1023u : 2047u)], 1u);
+            }
+            __syncthreads();
+            evict_pick<1024, GSR_EV_BINS>(s_hist, rank, s_tmp, bin, rank);
+            prefix = level == 2 ? (prefix << 10) | bin : (prefix << 11) | bin;
+        }
+        key = prefix; ties = rank;
+    }
+    uint32_t above = 0, equal = 0;
+    evict_emit_pass<1024, U>(a, 0, s, a.P, key, ties, s_n, above, equal);
 }
 
 struct RowTensor {
     const void* src; void* dst;
     const uint8_t* src_window; uint8_t* dst_window;          // codes of the 8-bit root: their windows (then a row's unit is one code)
     long long row;              // units of a row
-    uint32_t first, pad;
+    uint32_t first;             // its first workgroup
+    uint32_t magic;             // floor(x / row) = x magic / 2^32 for x < row + GSR_OPT_CHUNK; 0: a row of one, or too long for that
     int unit;                   // bytes of a unit: 1, 2, 4, 8 or 16
 };
-struct RowArgs { int count; uint32_t chunks; long long keep; const long long* kept; RowTensor t[GSR_OPT_MAX]; };
+struct RowArgs { int count; long long keep; const long long* kept; RowTensor t[GSR_OPT_MAX]; };
 
+// Where the units of a chunk come from: its first unit's row and column by one division, the others' by a multiplication.
+struct RowWalk {
+    const long long* kept; long long row; uint32_t col0, magic, last;          // last: the chunk's last unit
+    __device__ __forceinline__ RowWalk(const RowArgs& a, const RowTensor& t, long long base)
+    {
+        const long long left = a.keep * t.row - base, row0 = base / t.row;
+        kept = a.kept + row0; row = t.row; magic = t.magic;
+        col0 = (uint32_t)(base - row0 * t.row);
+        last = left < GSR_OPT_CHUNK ? (uint32_t)left - 1u : GSR_OPT_CHUNK - 1u;
+    }
+    // The sources of U units: all their rows' numbers are loaded before the first is used.
+    template <int U>
+    __device__ __forceinline__ void from(const uint32_t (&x)[U], long long (&e)[U]) const
+    {
+        uint32_t col[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t y = col0 + (x[u] < last ? x[u] : last);          // (behind the end: the last one again, not stored)
+            const uint32_t q = magic ? __umulhi(y, magic) : row == 1 ? y : y / (uint32_t)row;
+            col[u] = y - q * (uint32_t)row;
+            e[u] = kept[q];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) e[u] = e[u] * row + col[u];
+    }
+};
+
+// Consecutive lanes, consecutive units, GSR_EV_UNITS of a lane in flight; nothing is loaded under a condition, which would have each load
+// waited for where it stands (250 us for 1.35 M rows of 281 bytes, 154 so: 776 MB at 5.0 TB/s).  Staging the source's span in LDS, evicted
+// rows with it, was slower (280), a workgroup per 256 rows of all tensors as well (166).
 template <class T>
-__device__ __forceinline__ void evict_copy(const RowArgs& a, const RowTensor& t, uint32_t c)
+__device__ __forceinline__ void evict_chunk(const RowTensor& t, const RowWalk& w, long long base)
 {
-    const long long base = (long long)(c - t.first) * GSR_OPT_CHUNK, n = a.keep * t.row;
-    for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < n; k += GSR_OPT_THREADS) {
-        const long long i = base + k, row = i / t.row;
-        static_cast<T*>(t.dst)[i] = static_cast<const T*>(t.src)[a.kept[row] * t.row + (i - row * t.row)];
+    const T* src = static_cast<const T*>(t.src);
+    T* dst = static_cast<T*>(t.dst) + base;
+#pragma unroll 1
+    for (int h = 0; h < GSR_OPT_CHUNK / GSR_OPT_THREADS; h += GSR_EV_UNITS) {
+        uint32_t x[GSR_EV_UNITS];
+        long long e[GSR_EV_UNITS];
+        T v[GSR_EV_UNITS];
+#pragma unroll
+        for (int u = 0; u < GSR_EV_UNITS; u++) x[u] = (h + u) * GSR_OPT_THREADS + threadIdx.x;
+        w.from(x, e);
+#pragma unroll
+        for (int u = 0; u < GSR_EV_UNITS; u++) v[u] = src[e[u]];
+#pragma unroll
+        for (int u = 0; u < GSR_EV_UNITS; u++) if (x[u] <= w.last) dst[x[u]] = v[u];
     }
 }
 
 // Codes change their block with their row: the float's upper bits move into the new block's window, exactly, but for what lies under
-// that window (raised to its lowest value, as by the step).
-__device__ __forceinline__ void evict_codes(const RowArgs& a, const RowTensor& t, uint32_t c)
+// that window (raised to its lowest value, as by the step).  A wave per block of 256, four consecutive codes per lane.
+__device__ __forceinline__ void evict_codes(const RowTensor& t, const RowWalk& w, long long base)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
     const uint8_t* src = static_cast<const uint8_t*>(t.src);
-    uint8_t* dst = static_cast<uint8_t*>(t.dst);
-    const long long n = a.keep * t.row;
-    for (int b = wave; b < GSR_OPT_CHUNK / GSR_OPT_WINDOW; b += 4) {
-        const long long start = (long long)(c - t.first) * GSR_OPT_CHUNK + b * GSR_OPT_WINDOW;
-        if (start >= n) break;
-        uint32_t top[4], most = 0;
+    uint8_t* dst = static_cast<uint8_t*>(t.dst) + base;
+#pragma unroll 1
+    for (uint32_t b = threadIdx.x >> 6; b < GSR_OPT_CHUNK / GSR_OPT_WINDOW && b * GSR_OPT_WINDOW <= w.last; b += 4 * GSR_EV_BLOCKS) {
+        uint32_t x[4 * GSR_EV_BLOCKS], top[4 * GSR_EV_BLOCKS], window[4 * GSR_EV_BLOCKS];
+        long long e[4 * GSR_EV_BLOCKS];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            top[k] = 0;
-            const long long i = start + 4 * lane + k;
-            if (i < n) {
-                const long long row = i / t.row, e = a.kept[row] * t.row + (i - row * t.row);
-                const uint32_t code = src[e];
-                if (code) top[k] = code + 16u * t.src_window[e / GSR_OPT_WINDOW] + 1u;
-            }
-            most = top[k] > most ? top[k] : most;
-        }
-        const uint32_t w = opt_window(wave_max_u32(most) << 19), now = 16u * w + 1u;
+        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) x[k] = (b + 4 * (k >> 2)) * GSR_OPT_WINDOW + 4 * lane + (k & 3);
+        w.from(x, e);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const long long i = start + 4 * lane + k;
-            if (i < n) dst[i] = top[k] == 0u ? 0 : (uint8_t)(top[k] > now + 1u ? top[k] - now : 1u);
+        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) { top[k] = src[e[k]]; window[k] = t.src_window[e[k] / GSR_OPT_WINDOW]; }
+#pragma unroll
+        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) top[k] = top[k] && x[k] <= w.last ? top[k] + 16u * window[k] + 1u : 0u;
+#pragma unroll
+        for (int j = 0; j < GSR_EV_BLOCKS; j++) {
+            uint32_t most = 0, codes = 0;
+#pragma unroll
+            for (int k = 4 * j; k < 4 * j + 4; k++) most = top[k] > most ? top[k] : most;
+            const uint32_t nw = opt_window(wave_max_u32(most) << 19), now = 16u * nw + 1u, at = x[4 * j];
+#pragma unroll
+            for (int k = 0; k < 4; k++) codes |= (top[4 * j + k] == 0u ? 0u : top[4 * j + k] > now + 1u ? top[4 * j + k] - now : 1u) << (8 * k);
+            if (at + 3 <= w.last && opt_aligned4(dst)) *reinterpret_cast<uint32_t*>(dst + at) = codes;
+            else for (int k = 0; k < 4; k++) if (at + k <= w.last) dst[at + k] = (uint8_t)(codes >> (8 * k));
+            if (lane == 0 && at <= w.last) t.dst_window[(base + at) / GSR_OPT_WINDOW] = (uint8_t)nw;
         }
-        if (lane == 0) t.dst_window[start / GSR_OPT_WINDOW] = (uint8_t)w;
     }
 }
 
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_evict_rows(RowArgs a)
 {
-    for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-        const RowTensor& t = a.t[opt_find(a.t, a.count, c)];
-        if (t.src_window) evict_codes(a, t, c);
-        else if (t.unit == 16) evict_copy<uint4>(a, t, c);
-        else if (t.unit == 8) evict_copy<uint2>(a, t, c);
-        else if (t.unit == 4) evict_copy<uint32_t>(a, t, c);
-        else if (t.unit == 2) evict_copy<uint16_t>(a, t, c);
-        else evict_copy<uint8_t>(a, t, c);
-    }
+    const RowTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];
+    const long long base = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK;
+    const RowWalk w(a, t, base);
+    if (t.src_window) evict_codes(t, w, base);
+    else if (t.unit == 16) evict_chunk<opt_f4>(t, w, base);
+    else if (t.unit == 8) evict_chunk<opt_u2>(t, w, base);
+    else if (t.unit == 4) evict_chunk<uint32_t>(t, w, base);
+    else if (t.unit == 2) evict_chunk<uint16_t>(t, w, base);
+    else evict_chunk<uint8_t>(t, w, base);
 }
 
 }  // namespace gsr

@@ -5,10 +5,13 @@
 namespace {
 static_assert(sizeof(gsr::OptArgs) <= 4096 && sizeof(gsr::RowArgs) <= 4096 && sizeof(gsr::NormArgs) <= 4096 && sizeof(gsr::MomentArgs) <= 4096,
               "a launch's table must fit the kernel arguments");
-const long long kOptMaxElements = 1LL << 40;          // (chunks of a launch are counted in 32 bits)
-const int kOptGrid = 2048;                            // workgroups of a launch: eight per CU, each walks chunks
+const long long kOptMaxElements = 1LL << 36;          // (chunks of a launch are counted in 32 bits; 28 bytes each are more than the card has)
+const int kOptGrid = 2048;                            // workgroups of the norm's launches: eight per CU, each walks chunks
+// Past the caches from 256 MB on (what lies behind the L2): see opt_get.
+bool opt_stream(long long bytes) { return bytes > 256LL << 20; }
 bool opt_type_ok(int t) { return t == GSR_TYPE_F32 || t == GSR_TYPE_BF16 || t == GSR_TYPE_F16; }
 long long opt_size(int t) { return t == GSR_TYPE_F32 ? 4 : 2; }
+bool opt_aligned(const void* p, long long element) { return ((uintptr_t)p & (uintptr_t)(4 * element - 1)) == 0; }          // to four elements
 int opt_grid(uint32_t chunks) { return (int)std::max<uint32_t>(1u, std::min<uint32_t>(chunks, (uint32_t)kOptGrid)); }
 
 // Memory that one call writes: no two ranges of it, and no range that it only reads, may overlap.
@@ -70,26 +73,37 @@ int adamw_step(const gsr_adamw_args* a)
     k.clip = a->clip;
     const double span = eight ? (1.0 - a->beta1) / sqrt((1.0 - a->beta2) * (1.0 - a->beta1 * a->beta1 / a->beta2)) : 1.0;
     k.unit = (float)(span / 127.0); k.per_unit = (float)(127.0 / span);
-    k.count = 0; k.chunks = 0;
-    for (int i = 0; i < a->n_tensors; i++) {
-        const gsr_opt_tensor& t = a->tensors[i];
-        const uint32_t chunks = (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
-        OptTensor& o = k.t[k.count++];
-        o.p = t.param; o.g = t.grad; o.s0 = t.state0; o.s1 = t.state1; o.window = t.window; o.clock = t.clock; o.lr_device = t.lr_device;
-        o.lr = t.lr; o.decay = t.weight_decay; o.n = t.n; o.first = k.chunks;
-        o.key = a->seed * 0x9E3779B1u + (uint32_t)(i + 1) * 0x85EBCA77u;
-        o.types = t.param_type | t.grad_type << 4;
-        k.chunks += chunks;
-        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
-        if (!full && i + 1 < a->n_tensors) continue;
-        if (eight) {
-            hipLaunchKernelGGL(k_adamw8, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
-            LAUNCHCHK("k_adamw8");
-        } else {
-            hipLaunchKernelGGL(k_adamw, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
-            LAUNCHCHK("k_adamw");
+    for (int i = 0; i < a->n_tensors; ) {
+        const int count = std::min(GSR_OPT_MAX, a->n_tensors - i);
+        long long bytes = 0;
+        for (int j = i; j < i + count; j++) {
+            const gsr_opt_tensor& t = a->tensors[j];
+            bytes += t.n * (opt_size(t.param_type) + opt_size(t.grad_type) + (eight ? 2 : 8));
         }
-        k.count = 0; k.chunks = 0;
+        k.count = count;
+        uint32_t groups = 0;
+        for (int j = 0; j < count; j++, i++) {
+            const gsr_opt_tensor& t = a->tensors[i];
+            OptTensor& o = k.t[j];
+            o.p = t.param; o.g = t.grad; o.s0 = t.state0; o.s1 = t.state1; o.window = t.window; o.clock = t.clock; o.lr_device = t.lr_device;
+            o.lr = t.lr; o.decay = t.weight_decay; o.n = t.n; o.first = groups;
+            o.key = a->seed * 0x9E3779B1u + (uint32_t)(i + 1) * 0x85EBCA77u;
+            const bool aligned = opt_aligned(t.param, opt_size(t.param_type)) && opt_aligned(t.grad, opt_size(t.grad_type)) &&
+                                 opt_aligned(t.state0, eight ? 1 : 4) && opt_aligned(t.state1, eight ? 1 : 4);
+            o.types = t.param_type | t.grad_type << 4 | (aligned ? GSR_T_ALIGNED : 0);
+            groups += (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+        }
+        const dim3 grid(std::max(1u, groups)), block(GSR_OPT_THREADS);
+        const bool stream_past = opt_stream(bytes);
+        if (eight && stream_past) hipLaunchKernelGGL(k_adamw8<true>, grid, block, 0, st, k);
+        else if (eight) hipLaunchKernelGGL(k_adamw8<false>, grid, block, 0, st, k);
+        else if (stream_past) hipLaunchKernelGGL(k_adamw<true>, grid, block, 0, st, k);
+        else hipLaunchKernelGGL(k_adamw<false>, grid, block, 0, st, k);
+        LAUNCHCHK(eight ? "k_adamw8" : "k_adamw");
+        if (grid.x > GSR_OPT_TICKETS) {
+            hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(64), 0, st, k);
+            LAUNCHCHK("k_adamw_advance");
+        }
     }
     return 0;
 }
@@ -119,19 +133,21 @@ int adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1,
     if (rc != GSR_OK) return rc;
     MomentArgs k;
     k.unit = (float)((1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)) / 127.0);
-    k.type = type; k.count = 0; k.chunks = 0;
+    k.type = type; k.count = 0;
+    uint32_t groups = 0;
     for (int i = 0; i < n_tensors; i++) {
         const gsr_moment_tensor& t = tensors[i];
         if (t.n > 0) {
             MomentTensor& o = k.t[k.count++];
-            o.rms = t.rms; o.ratio = t.ratio; o.window = t.window; o.exp_avg = t.exp_avg_out; o.root = t.rms_out; o.n = t.n; o.first = k.chunks;
-            k.chunks += (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+            o.rms = t.rms; o.ratio = t.ratio; o.window = t.window; o.exp_avg = t.exp_avg_out; o.root = t.rms_out; o.n = t.n; o.first = groups;
+            o.aligned = opt_aligned(t.rms, 1) && opt_aligned(t.ratio, 1) && opt_aligned(t.exp_avg_out, opt_size(type)) && opt_aligned(t.rms_out, opt_size(type));
+            groups += (uint32_t)((t.n + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
         }
-        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
+        const bool full = k.count == GSR_OPT_MAX || groups > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
         if (k.count == 0 || (!full && i + 1 < n_tensors)) continue;
-        hipLaunchKernelGGL(k_moments8, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+        hipLaunchKernelGGL(k_moments8, dim3(groups), dim3(GSR_OPT_THREADS), 0, st, k);
         LAUNCHCHK("k_moments8");
-        k.count = 0; k.chunks = 0;
+        k.count = 0; groups = 0;
     }
     return 0;
 }
@@ -160,7 +176,7 @@ int grad_norm(int n_tensors, const void* const* grads, const long long* numels, 
     int sums = 0;
     for (int i = 0; i < n_tensors; i++) {
         if (numels[i] > 0) {
-            k.t[k.count++] = {grads[i], numels[i], k.chunks, types[i]};
+            k.t[k.count++] = {grads[i], numels[i], k.chunks, types[i] | (opt_aligned(grads[i], opt_size(types[i])) ? GSR_T_ALIGNED : 0)};
             k.chunks += (uint32_t)((numels[i] + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
         }
         const bool full = k.count == GSR_NORM_MAX || k.chunks > 0x70000000u - (uint32_t)(kOptMaxElements / GSR_OPT_CHUNK);
@@ -177,11 +193,12 @@ int grad_norm(int n_tensors, const void* const* grads, const long long* numels, 
     return 0;
 }
 
-struct EvictWs { uint32_t* hist; uint2* counts; float* total; };
+struct EvictWs { uint32_t* hist; uint32_t* found; uint2* counts; float* total; };
 size_t carve_evict(char* base, int P, EvictWs& w)
 {
     Carver c(base);
     w.hist = c.take<uint32_t>(3 * GSR_EV_BINS);
+    w.found = c.take<uint32_t>(6);
     w.counts = c.take<uint2>(GSR_EV_TILES);
     w.total = c.take<float>(P > 0 ? (size_t)P : 1);
     return c.size();
@@ -197,7 +214,7 @@ int evict_rows(const gsr_evict_args* a)
     if (a->n_tensors > 0 && !a->tensors) return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
     for (int i = 0; i < a->n_tensors; i++) {
         const gsr_row_tensor& t = a->tensors[i];
-        if (t.row_bytes < 0 || t.row_bytes * (long long)a->P > 4 * kOptMaxElements || t.row_bytes > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_evict_rows: bad row size%s", "");
+        if (t.row_bytes < 0 || t.row_bytes > 0x7fffffffLL || t.row_bytes > 4 * kOptMaxElements / std::max(1, a->P)) return fail(GSR_E_INVALID, "gsr_evict_rows: bad row size%s", "");
         if (a->keep > 0 && t.row_bytes > 0 && (!t.src || !t.dst || (t.src_window != nullptr) != (t.dst_window != nullptr)))
             return fail(GSR_E_INVALID, "gsr_evict_rows: NULL pointer%s", "");
     }
@@ -223,45 +240,55 @@ int evict_rows(const gsr_evict_args* a)
     carve_evict(ws, a->P, w);
     EvictArgs e;
     e.P = a->P; e.views = a->n_views; e.old = a->P - a->recent; e.k = a->keep - a->recent; e.decay = a->decay;
-    e.scores = a->scores; e.weights = a->weights; e.total = w.total; e.hist = w.hist; e.counts = w.counts;
+    e.scores = a->scores; e.weights = a->weights; e.total = w.total; e.hist = w.hist; e.found = w.found; e.counts = w.counts;
     e.kept = a->kept; e.scores_out = a->scores_out;
-    const int per = (int)(((long long)a->P + GSR_EV_TILES - 1) / GSR_EV_TILES);
-    e.tile_rows = (int)std::max<long long>(1024, ((long long)per + 255) / 256 * 256);
-    e.tiles = (int)(((long long)a->P + e.tile_rows - 1) / e.tile_rows);
-    ClearRanges cr = {};
-    cr.p[0] = w.hist; cr.n[0] = 3 * GSR_EV_BINS;
-    hipLaunchKernelGGL(k_refine_init, dim3(3 * GSR_EV_BINS / GSR_BLOCK), dim3(GSR_BLOCK), 0, st, cr, PoseLoadArgs{});
-    LAUNCHCHK("k_refine_init");
-    const int blocks = (int)std::min<long long>(((long long)a->P + 255) / 256, 1024);
-    hipLaunchKernelGGL(k_evict_scores, dim3(blocks), dim3(256), 0, st, e);
-    LAUNCHCHK("k_evict_scores");
-    if (e.k > 0 && e.k < e.old) {
-        hipLaunchKernelGGL(k_evict_hist<2>, dim3(blocks), dim3(256), 0, st, e);
-        LAUNCHCHK("k_evict_hist<2>");
-        hipLaunchKernelGGL(k_evict_hist<3>, dim3(blocks), dim3(256), 0, st, e);
-        LAUNCHCHK("k_evict_hist<3>");
+    if (a->P <= GSR_EV_SMALL) {          // one workgroup, one launch: at 2000 rows 12 us for the six's 25
+        hipLaunchKernelGGL(k_evict_small, dim3(1), dim3(1024), 0, st, e);
+        LAUNCHCHK("k_evict_small");
+    } else {
+        const long long tiles = std::min<long long>(((long long)a->P + GSR_EV_TILE - 1) / GSR_EV_TILE, GSR_EV_TILES), per = ((long long)a->P + tiles - 1) / tiles;
+        e.tile_rows = (int)((per + GSR_EV_TILE - 1) / GSR_EV_TILE * GSR_EV_TILE);
+        const int n_tiles = (int)(((long long)a->P + e.tile_rows - 1) / e.tile_rows);
+        if (e.k > 0 && e.k < e.old) {
+            ClearRanges cr = {};
+            cr.p[0] = w.hist; cr.n[0] = 3 * GSR_EV_BINS;
+            hipLaunchKernelGGL(k_refine_init, dim3(3 * GSR_EV_BINS / GSR_BLOCK), dim3(GSR_BLOCK), 0, st, cr, PoseLoadArgs{});
+            LAUNCHCHK("k_refine_init");
+        }
+        hipLaunchKernelGGL(k_evict_scores, dim3((unsigned)std::min<long long>(((long long)a->P + 2047) / 2048, 256)), dim3(512), 0, st, e);
+        LAUNCHCHK("k_evict_scores");
+        if (e.k > 0 && e.k < e.old) {
+            const dim3 blocks((unsigned)std::min<long long>(((long long)a->P + 8191) / 8192, 256));
+            hipLaunchKernelGGL(k_evict_hist<2>, blocks, dim3(1024), 0, st, e);
+            LAUNCHCHK("k_evict_hist<2>");
+            hipLaunchKernelGGL(k_evict_hist<3>, blocks, dim3(1024), 0, st, e);
+            LAUNCHCHK("k_evict_hist<3>");
+        }
+        hipLaunchKernelGGL(k_evict_count, dim3(n_tiles), dim3(256), 0, st, e);
+        LAUNCHCHK("k_evict_count");
+        hipLaunchKernelGGL(k_evict_emit, dim3(n_tiles), dim3(256), 0, st, e);
+        LAUNCHCHK("k_evict_emit");
     }
-    hipLaunchKernelGGL(k_evict_count, dim3(e.tiles), dim3(256), 0, st, e);
-    LAUNCHCHK("k_evict_count");
-    hipLaunchKernelGGL(k_evict_emit, dim3(e.tiles), dim3(256), 0, st, e);
-    LAUNCHCHK("k_evict_emit");
     RowArgs k;
-    k.keep = a->keep; k.kept = a->kept; k.count = 0; k.chunks = 0;
+    k.keep = a->keep; k.kept = a->kept; k.count = 0;
+    uint32_t groups = 0;
     for (int i = 0; i < a->n_tensors; i++) {
         const gsr_row_tensor& t = a->tensors[i];
         if (t.row_bytes > 0) {
             RowTensor& o = k.t[k.count++];
-            o.src = t.src; o.dst = t.dst; o.src_window = t.src_window; o.dst_window = t.dst_window; o.first = k.chunks; o.pad = 0;
             const uintptr_t bits = (uintptr_t)t.src | (uintptr_t)t.dst | (uintptr_t)t.row_bytes;
+            o.src = t.src; o.dst = t.dst; o.src_window = t.src_window; o.dst_window = t.dst_window; o.first = groups;
             o.unit = t.src_window ? 1 : (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
             o.row = t.row_bytes / o.unit;
-            k.chunks += (uint32_t)((o.row * a->keep + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+            // y ceil(2^32 / row) exceeds y 2^32 / row by less than y: the quotient is right while y row < 2^32
+            o.magic = o.row > 1 && (o.row + GSR_OPT_CHUNK) * o.row < (1LL << 32) ? (uint32_t)(((1LL << 32) + o.row - 1) / o.row) : 0u;
+            groups += (uint32_t)((o.row * a->keep + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
         }
-        const bool full = k.count == GSR_OPT_MAX || k.chunks > 0x40000000u;
+        const bool full = k.count == GSR_OPT_MAX || groups > 0x20000000u;
         if (k.count == 0 || (!full && i + 1 < a->n_tensors)) continue;
-        hipLaunchKernelGGL(k_evict_rows, dim3(opt_grid(k.chunks)), dim3(GSR_OPT_THREADS), 0, st, k);
+        hipLaunchKernelGGL(k_evict_rows, dim3(groups), dim3(GSR_OPT_THREADS), 0, st, k);
         LAUNCHCHK("k_evict_rows");
-        k.count = 0; k.chunks = 0;
+        k.count = 0; groups = 0;
     }
     return 0;
 }
