@@ -198,7 +198,9 @@ __device__ __forceinline__ void opt_begin(const OptArgs& a, const OptTensor& t, 
     r.key = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t.key + (uint32_t)(t.clock[2] + 1.0)));
     r.ticket = 0;
     if (gridDim.x > GSR_OPT_TICKETS) return;
-    __syncthreads();          // all four waves have the clock
+    // the values, so that the clock has arrived, and not only been asked for, before the barrier
+    asm volatile("" : : "s"(__float_as_uint(r.shrink)), "s"(__float_as_uint(r.rate)), "s"(__float_as_uint(r.unbias)), "s"(r.key) : "memory");
+    __syncthreads();          // all four waves have it
     if (threadIdx.x == 0) r.ticket = __hip_atomic_fetch_add(reinterpret_cast<unsigned*>(a.t[0].clock + 3), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void opt_advance(const OptArgs& a)          // one wave
@@ -519,6 +521,7 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
 
 #define GSR_EV_UNITS 16         // units of a lane whose loads are in flight together (4: 178 us for 1.35 M rows of 281 bytes, 8: 173, 16: 154)
 #define GSR_EV_BLOCKS 4         // blocks of codes likewise
+#define GSR_EV_CHUNK 8192       // units of one byte that a workgroup copies (of others GSR_OPT_CHUNK)
 #define GSR_EV_BINS 2048
 #define GSR_EV_COPIES 8         // of the first histogram in LDS: its bins are exponents, a wave's lanes meet in few of them
 #define GSR_EV_TILE 1024        // rows of a tile, or a multiple of it
@@ -827,35 +830,61 @@ struct RowTensor {
     const uint8_t* src_window; uint8_t* dst_window;          // codes of the 8-bit root: their windows (then a row's unit is one code)
     long long row;              // units of a row
     uint32_t first;             // its first workgroup
-    uint32_t magic;             // floor(x / row) = x magic / 2^32 for x < row + GSR_OPT_CHUNK; 0: a row of one, or too long for that
+    uint32_t magic;             // floor(x / row) = x magic / 2^32 for x < row + GSR_EV_CHUNK; 0: a row of one, or too long for that
     int unit;                   // bytes of a unit: 1, 2, 4, 8 or 16
+    int large;                  // the source has 4 GB or more
 };
 struct RowArgs { int count; long long keep; const long long* kept; RowTensor t[GSR_OPT_MAX]; };
 
-// Where the units of a chunk come from: its first unit's row and column by one division, the others' by a multiplication.
+// Where the units of a chunk come from: its first unit's row and column by one division, the others' by a multiplication.  OFF: the type of
+// the sources' byte offsets.
+template <class OFF>
 struct RowWalk {
-    const long long* kept; long long row; uint32_t col0, magic, last;          // last: the chunk's last unit
-    __device__ __forceinline__ RowWalk(const RowArgs& a, const RowTensor& t, long long base)
+    const char* kept; OFF row_bytes; uint32_t row, col0, magic, last;          // kept: of the chunk's first row on; last: the chunk's last unit
+    __device__ __forceinline__ RowWalk(const RowArgs& a, const RowTensor& t, long long base, uint32_t chunk)
     {
         const long long left = a.keep * t.row - base, row0 = base / t.row;
-        kept = a.kept + row0; row = t.row; magic = t.magic;
+        kept = reinterpret_cast<const char*>(a.kept + row0); row = (uint32_t)t.row; magic = t.magic;
+        row_bytes = (OFF)t.row * (OFF)t.unit;
         col0 = (uint32_t)(base - row0 * t.row);
-        last = left < GSR_OPT_CHUNK ? (uint32_t)left - 1u : GSR_OPT_CHUNK - 1u;
+        last = left < chunk ? (uint32_t)left - 1u : chunk - 1u;
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t x, uint32_t& col) const          // which row of the chunk's, and which unit in it
+    {
+        const uint32_t y = col0 + (x < last ? x : last);          // (behind the end: the last one again, not stored)
+        const uint32_t q = magic ? __umulhi(y, magic) : row == 1 ? y : y / row;
+        col = y - q * row;
+        return q;
+    }
+    __device__ __forceinline__ OFF number(uint32_t q) const          // of the chunk's q-th row (int64 in memory, of a chunk under 2^32 bytes)
+    {
+        return (OFF)*reinterpret_cast<const OFF*>(kept + (uint32_t)(8u * q));
     }
     // The sources of U units: all their rows' numbers are loaded before the first is used.
-    template <int U>
-    __device__ __forceinline__ void from(const uint32_t (&x)[U], long long (&e)[U]) const
+    template <int UNIT, int U>
+    __device__ __forceinline__ void from(const uint32_t (&x)[U], OFF (&e)[U]) const
     {
         uint32_t col[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint32_t y = col0 + (x[u] < last ? x[u] : last);          // (behind the end: the last one again, not stored)
-            const uint32_t q = magic ? __umulhi(y, magic) : row == 1 ? y : y / (uint32_t)row;
-            col[u] = y - q * (uint32_t)row;
-            e[u] = kept[q];
-        }
+        for (int u = 0; u < U; u++) e[u] = number(place(x[u], col[u]));
 #pragma unroll
-        for (int u = 0; u < U; u++) e[u] = e[u] * row + col[u];
+        for (int u = 0; u < U; u++) e[u] = e[u] * row_bytes + (OFF)(col[u] * UNIT);
+    }
+    // The same for groups of four consecutive bytes of rows of three or more, which lie in two rows at most: one division, two loads and two
+    // products a group.  wrap: this unit is in the second row.
+    template <int U>
+    __device__ __forceinline__ void fours(const uint32_t (&x)[U], OFF (&e)[U], bool (&wrap)[U]) const
+    {
+        uint32_t q[U / 4], col[U / 4];
+        OFF first[U / 4], second[U / 4];
+#pragma unroll
+        for (int j = 0; j < U / 4; j++) q[j] = place(x[4 * j], col[j]);
+#pragma unroll
+        for (int j = 0; j < U / 4; j++) { first[j] = number(q[j]); second[j] = number(q[j] + (col[j] + 3 >= row ? 1 : 0)); }
+#pragma unroll
+        for (int j = 0; j < U / 4; j++) { first[j] = first[j] * row_bytes + col[j]; second[j] = second[j] * row_bytes + (OFF)col[j] - (OFF)row; }
+#pragma unroll
+        for (int u = 0; u < U; u++) { wrap[u] = col[u / 4] + (u & 3) >= row; e[u] = (wrap[u] ? second[u / 4] : first[u / 4]) + (OFF)(u & 3); }
     }
 };
 
@@ -863,54 +892,84 @@ struct RowWalk {
 // waited for where it stands (250 us for 1.35 M rows of 281 bytes, 154 so: 776 MB at 5.0 TB/s).  Staging the source's span in LDS, evicted
 // rows with it, was slower (280), a workgroup per 256 rows of all tensors as well (166).
 template <class T>
-__device__ __forceinline__ void evict_chunk(const RowTensor& t, const RowWalk& w, long long base)
+__device__ __forceinline__ void evict_chunk(const RowArgs& a, const RowTensor& t, long long base, uint32_t chunk)
 {
-    const T* src = static_cast<const T*>(t.src);
+    constexpr int U = sizeof(T) <= 4 ? GSR_EV_UNITS : GSR_EV_UNITS * 4 / (int)sizeof(T);          // the same bytes, and registers, for every unit
+    typedef unsigned long long OFF;          // (no register is scarce here: 32 bits gain nothing, 160 us for 154)
+    const RowWalk<OFF> w(a, t, base, chunk);
+    const char* src = static_cast<const char*>(t.src);
     T* dst = static_cast<T*>(t.dst) + base;
 #pragma unroll 1
-    for (int h = 0; h < GSR_OPT_CHUNK / GSR_OPT_THREADS; h += GSR_EV_UNITS) {
-        uint32_t x[GSR_EV_UNITS];
-        long long e[GSR_EV_UNITS];
-        T v[GSR_EV_UNITS];
+    for (int h = 0; h < GSR_OPT_CHUNK / GSR_OPT_THREADS; h += U) {
+        uint32_t x[U];
+        OFF e[U];
+        T v[U];
 #pragma unroll
-        for (int u = 0; u < GSR_EV_UNITS; u++) x[u] = (h + u) * GSR_OPT_THREADS + threadIdx.x;
-        w.from(x, e);
+        for (int u = 0; u < U; u++) x[u] = (h + u) * GSR_OPT_THREADS + threadIdx.x;
+        w.template from<(int)sizeof(T)>(x, e);
 #pragma unroll
-        for (int u = 0; u < GSR_EV_UNITS; u++) v[u] = src[e[u]];
+        for (int u = 0; u < U; u++) v[u] = *reinterpret_cast<const T*>(src + e[u]);
 #pragma unroll
-        for (int u = 0; u < GSR_EV_UNITS; u++) if (x[u] <= w.last) dst[x[u]] = v[u];
+        for (int u = 0; u < U; u++) if (x[u] <= w.last) dst[x[u]] = v[u];
     }
 }
 
-// Codes change their block with their row: the float's upper bits move into the new block's window, exactly, but for what lies under
-// that window (raised to its lowest value, as by the step).  A wave per block of 256, four consecutive codes per lane.
-__device__ __forceinline__ void evict_codes(const RowTensor& t, const RowWalk& w, long long base)
+// Units of one byte: four consecutive ones per lane, a wave per 256, GSR_EV_BLOCKS of those in flight; offsets of 32 bits where the source
+// has less than 4 GB (1.35 M rows of 180 bytes: 205 us, 240 with 64; as codes 240, 294).
+//
+// Codes of the 8-bit root change their block with their row: the float's upper bits move into the new block's window, exactly, but for
+// what lies under that window (raised to its lowest value, as by the step).
+template <bool CODES, class OFF>
+__device__ __forceinline__ void evict_bytes(const RowArgs& a, const RowTensor& t, long long base, uint32_t chunk)
 {
+    const RowWalk<OFF> w(a, t, base, chunk);
     const int lane = threadIdx.x & 63;
     const uint8_t* src = static_cast<const uint8_t*>(t.src);
     uint8_t* dst = static_cast<uint8_t*>(t.dst) + base;
 #pragma unroll 1
-    for (uint32_t b = threadIdx.x >> 6; b < GSR_OPT_CHUNK / GSR_OPT_WINDOW && b * GSR_OPT_WINDOW <= w.last; b += 4 * GSR_EV_BLOCKS) {
-        uint32_t x[4 * GSR_EV_BLOCKS], top[4 * GSR_EV_BLOCKS], window[4 * GSR_EV_BLOCKS];
-        long long e[4 * GSR_EV_BLOCKS];
+    for (uint32_t b = threadIdx.x >> 6; b * GSR_OPT_WINDOW <= w.last; b += 4 * GSR_EV_BLOCKS) {
+        constexpr int U = 4 * GSR_EV_BLOCKS;
+        uint32_t x[U], v[U], window[U];
+        OFF e[U];
 #pragma unroll
-        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) x[k] = (b + 4 * (k >> 2)) * GSR_OPT_WINDOW + 4 * lane + (k & 3);
-        w.from(x, e);
+        for (int k = 0; k < U; k++) x[k] = (b + 4 * (k >> 2)) * GSR_OPT_WINDOW + 4 * lane + (k & 3);
+        if (w.row >= 3 && (b + U) * GSR_OPT_WINDOW <= w.last + 1u) {
+            // Rows ascend, so four units' sources do: the four bytes from the first and the four up to the last lie inside the tensor and hold them all.
+            uint32_t lo[GSR_EV_BLOCKS], hi[GSR_EV_BLOCKS];
+            bool wrap[U];
+            w.fours(x, e, wrap);
 #pragma unroll
-        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) { top[k] = src[e[k]]; window[k] = t.src_window[e[k] / GSR_OPT_WINDOW]; }
+            for (int j = 0; j < GSR_EV_BLOCKS; j++) { __builtin_memcpy(&lo[j], src + e[4 * j], 4); __builtin_memcpy(&hi[j], src + (e[4 * j + 3] - 3), 4); }
 #pragma unroll
-        for (int k = 0; k < 4 * GSR_EV_BLOCKS; k++) top[k] = top[k] && x[k] <= w.last ? top[k] + 16u * window[k] + 1u : 0u;
+            for (int k = 0; k < U; k++) v[k] = ((wrap[k] ? hi[k / 4] : lo[k / 4]) >> (8 * (k & 3))) & 255u;
+        } else {
+            w.template from<1>(x, e);
+#pragma unroll
+            for (int k = 0; k < U; k++) v[k] = src[e[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) window[k] = CODES ? t.src_window[e[k] / GSR_OPT_WINDOW] : 0u;
 #pragma unroll
         for (int j = 0; j < GSR_EV_BLOCKS; j++) {
-            uint32_t most = 0, codes = 0;
+            const uint32_t at = x[4 * j];
+            uint32_t bytes = 0;
+            if (CODES) {
+                uint32_t top[4], most = 0;
 #pragma unroll
-            for (int k = 4 * j; k < 4 * j + 4; k++) most = top[k] > most ? top[k] : most;
-            const uint32_t nw = opt_window(wave_max_u32(most) << 19), now = 16u * nw + 1u, at = x[4 * j];
+                for (int k = 0; k < 4; k++) {
+                    top[k] = v[4 * j + k] && x[4 * j + k] <= w.last ? v[4 * j + k] + 16u * window[4 * j + k] + 1u : 0u;
+                    most = top[k] > most ? top[k] : most;
+                }
+                const uint32_t nw = opt_window(wave_max_u32(most) << 19), now = 16u * nw + 1u;
 #pragma unroll
-            for (int k = 0; k < 4; k++) codes |= (top[4 * j + k] == 0u ? 0u : top[4 * j + k] > now + 1u ? top[4 * j + k] - now : 1u) << (8 * k);
-            if (at + 3 <= w.last && opt_aligned4(dst)) *reinterpret_cast<uint32_t*>(dst + at) = codes;
-            else for (int k = 0; k < 4; k++) if (at + k <= w.last) dst[at + k] = (uint8_t)(codes >> (8 * k));
-            if (lane == 0 && at <= w.last) t.dst_window[(base + at) / GSR_OPT_WINDOW] = (uint8_t)nw;
+                for (int k = 0; k < 4; k++) bytes |= (top[k] == 0u ? 0u : top[k] > now + 1u ? top[k] - now : 1u) << (8 * k);
+                if (lane == 0 && at <= w.last) t.dst_window[(base + at) / GSR_OPT_WINDOW] = (uint8_t)nw;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) bytes |= v[4 * j + k] << (8 * k);
+            }
+            if (at + 3 <= w.last && opt_aligned4(dst)) *reinterpret_cast<uint32_t*>(dst + at) = bytes;
+            else for (int k = 0; k < 4; k++) if (at + k <= w.last) dst[at + k] = (uint8_t)(bytes >> (8 * k));
         }
     }
 }
@@ -918,14 +977,15 @@ __device__ __forceinline__ void evict_codes(const RowTensor& t, const RowWalk& w
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_evict_rows(RowArgs a)
 {
     const RowTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];
-    const long long base = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK;
-    const RowWalk w(a, t, base);
-    if (t.src_window) evict_codes(t, w, base);
-    else if (t.unit == 16) evict_chunk<opt_f4>(t, w, base);
-    else if (t.unit == 8) evict_chunk<opt_u2>(t, w, base);
-    else if (t.unit == 4) evict_chunk<uint32_t>(t, w, base);
-    else if (t.unit == 2) evict_chunk<uint16_t>(t, w, base);
-    else evict_chunk<uint8_t>(t, w, base);
+    const uint32_t chunk = t.unit == 1 ? GSR_EV_CHUNK : GSR_OPT_CHUNK;
+    const long long base = (long long)(blockIdx.x - t.first) * chunk;
+    if (t.src_window) { if (t.large) evict_bytes<true, unsigned long long>(a, t, base, chunk); else evict_bytes<true, uint32_t>(a, t, base, chunk); }
+    else if (t.unit == 16) evict_chunk<opt_f4>(a, t, base, chunk);
+    else if (t.unit == 8) evict_chunk<opt_u2>(a, t, base, chunk);
+    else if (t.unit == 4) evict_chunk<uint32_t>(a, t, base, chunk);
+    else if (t.unit == 2) evict_chunk<uint16_t>(a, t, base, chunk);
+    else if (t.large) evict_bytes<false, unsigned long long>(a, t, base, chunk);
+    else evict_bytes<false, uint32_t>(a, t, base, chunk);
 }
 
 }  // namespace gsr

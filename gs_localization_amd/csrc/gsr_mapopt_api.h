@@ -242,7 +242,7 @@ int evict_rows(const gsr_evict_args* a)
     e.P = a->P; e.views = a->n_views; e.old = a->P - a->recent; e.k = a->keep - a->recent; e.decay = a->decay;
     e.scores = a->scores; e.weights = a->weights; e.total = w.total; e.hist = w.hist; e.found = w.found; e.counts = w.counts;
     e.kept = a->kept; e.scores_out = a->scores_out;
-    if (a->P <= GSR_EV_SMALL) {          // one workgroup, one launch: at 2000 rows 12 us for the six's 25
+    if (a->P <= GSR_EV_SMALL) {          // one workgroup, one launch: at 2000 rows 15 us for the six's 25
         hipLaunchKernelGGL(k_evict_small, dim3(1), dim3(1024), 0, st, e);
         LAUNCHCHK("k_evict_small");
     } else {
@@ -280,9 +280,11 @@ int evict_rows(const gsr_evict_args* a)
             o.src = t.src; o.dst = t.dst; o.src_window = t.src_window; o.dst_window = t.dst_window; o.first = groups;
             o.unit = t.src_window ? 1 : (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
             o.row = t.row_bytes / o.unit;
+            o.large = t.row_bytes * a->P >= (1LL << 32);
             // y ceil(2^32 / row) exceeds y 2^32 / row by less than y: the quotient is right while y row < 2^32
-            o.magic = o.row > 1 && (o.row + GSR_OPT_CHUNK) * o.row < (1LL << 32) ? (uint32_t)(((1LL << 32) + o.row - 1) / o.row) : 0u;
-            groups += (uint32_t)((o.row * a->keep + GSR_OPT_CHUNK - 1) / GSR_OPT_CHUNK);
+            o.magic = o.row > 1 && (o.row + GSR_EV_CHUNK) * o.row < (1LL << 32) ? (uint32_t)(((1LL << 32) + o.row - 1) / o.row) : 0u;
+            const long long chunk = o.unit == 1 ? GSR_EV_CHUNK : GSR_OPT_CHUNK;
+            groups += (uint32_t)((o.row * a->keep + chunk - 1) / chunk);
         }
         const bool full = k.count == GSR_OPT_MAX || groups > 0x20000000u;
         if (k.count == 0 || (!full && i + 1 < a->n_tensors)) continue;

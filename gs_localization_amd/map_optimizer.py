@@ -10,7 +10,8 @@ gaussian_model.py:269-328 rewrites its state whenever splats are pruned or added
   grad_norm, adamw_step, adamw_step_8bit, moments_8bit, evict_rows      the operators by themselves
   compositing_weights                                                   what evict_rows accumulates, from the rasterizer
 
-No entry point reads anything back, and each runs on its tensors' device and that device's current stream.  Nothing falls back to torch
+No entry point reads anything back, and each runs on its tensors' device and that device's current stream; two steps of the same tensors
+must not overlap, as with any operation in place.  Nothing falls back to torch
 or to the CPU: tensors elsewhere are refused.  Tensors that a step writes must be contiguous and must not overlap (refused); the
 step counts live on the device, so a captured graph counts on when it is replayed."""
 import ctypes as C
@@ -291,6 +292,9 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm, self.seed, self.last_norm = max_norm, int(seed), None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
+    def __getstate__(self):          # (copies and pickles)
+        return dict(super().__getstate__(), max_norm=self.max_norm, seed=self.seed, last_norm=None)
+
     def add_param_group(self, group):
         super().add_param_group(group)
         g = self.param_groups[-1]
@@ -378,6 +382,7 @@ class AdamW(torch.optim.Optimizer):
                 if not torch.is_tensor(st["step"]) or st["step"].numel() == 1:
                     t = float(st["step"])
                     st["step"] = torch.tensor([g["betas"][0] ** t, g["betas"][1] ** t, t, 0.0], dtype=torch.float64, device=p.device)
+                st["step"] = st["step"].double()
                 if b == 32:
                     st["exp_avg"], st["exp_avg_sq"] = st["exp_avg"].float(), st["exp_avg_sq"].float()
                 self.state[p] = st

@@ -746,3 +746,124 @@ def test_c_program_without_python(tmp_path):
     subprocess.check_call(["gcc", "-std=c99", "-Wall", "-I" + os.path.join(root, "include"), str(src), "-L" + lib, "-lgsr_hip", "-L/opt/rocm/lib", "-lamdhip64",
                            "-Wl,-rpath," + lib + ":/opt/rocm/lib", "-o", str(tmp_path / "a")])
     subprocess.check_call([str(tmp_path / "a")])
+
+
+# ---- where the launches change their shape ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [511 * 4096, 512 * 4096, 512 * 4096 + 1, 520 * 4096 + 3, 17_000_003, 27_000_002])
+def test_large_launches(bits, n):
+    """around 512 workgroups (the clock's own launch from there on) and past 256 MB (non-temporal): elements of the first, some middle and the last
+    workgroups against the oracle, and the clock, over three steps"""
+    gen = torch.Generator(device=DEV).manual_seed(30)
+    p, g = torch.randn(n, generator=gen, device=DEV), torch.randn(n, generator=gen, device=DEV)
+    betas, ck = (0.9, 0.999), clocks(2, 0, (0.9, 0.999))
+    small = [torch.ones(5, device=DEV), torch.ones(5, device=DEV)]
+    if bits == 32:
+        st = [torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)]
+        st5 = [torch.zeros(5, device=DEV), torch.zeros(5, device=DEV)]
+    else:
+        like = lambda k: [torch.zeros(k, dtype=torch.uint8, device=DEV), torch.zeros(k, dtype=torch.int8, device=DEV), torch.zeros((k + 255) // 256, dtype=torch.uint8, device=DEV)]      # noqa: E731
+        st, st5 = like(n), like(5)
+    look = [slice(0, 1024), slice(256 * (n // 512), 256 * (n // 512) + 2048), slice((n - 3000) // 256 * 256, n)]
+    for t in (1, 2, 3):
+        before = [[x[s].clone() for x in (p, g, *st[:2])] + ([] if bits == 32 else [st[2][s.start // 256:(s.stop + 255) // 256].clone()]) for s in look]
+        if bits == 32:
+            MO().adamw_step([small[0], p], [small[1], g], [st5[0], st[0]], [st5[1], st[1]], ck, lr=0.01)
+        else:
+            MO().adamw_step_8bit([small[0], p], [small[1], g], [st5[0], st[0]], [st5[1], st[1]], [st5[2], st[2]], ck, lr=0.01, seed=1)
+        for c in ck:
+            assert c.tolist() == [betas[0] * (1.0 if t == 1 else c_prev[0]), betas[1] * (1.0 if t == 1 else c_prev[1]), t, 0.0]
+        c_prev = ck[0].tolist()
+        for s, b in zip(look, before):
+            if bits == 32:
+                p1, m1, v1, scale = O.adamw(n64(b[0]), n64(b[1]), n64(b[2]), n64(b[3]), t, 0.01, betas, 1e-8, 0.0)
+                assert (np.abs(n64(st[1][s]) - v1) <= 7 * E * v1).all()
+                assert (np.abs(n64(p[s]) - p1) <= bound32(p1, m1, v1, scale, 0.01, 0.0, torch.float32)).all()
+            else:
+                u = O.decode(b[2].cpu().numpy(), b[4].cpu().numpy())
+                m = n64(b[3]) / 127 * O.span(*betas) * u
+                p1, m1, v1, scale = O.adamw(n64(b[0]), n64(b[1]), m, u * u, t, 0.01, betas, 1e-8, 0.0)
+                assert (np.abs(n64(p[s]) - p1) <= bound32(p1, m1, v1, scale * 1.2, 0.01, 0.0, torch.float32)).all()
+                root = O.decode(st[0][s].cpu().numpy(), st[2][s.start // 256:(s.stop + 255) // 256].cpu().numpy())
+                # a root is stored to a sixteenth of its binade, or as its window's lowest value
+                low = np.repeat(root[: len(root) // 256 * 256].reshape(-1, 256).max(1) * 2.0 ** -14, 256)
+                k = low.size
+                assert (np.abs(root[:k] - np.sqrt(v1)[:k]) <= np.maximum(np.sqrt(v1)[:k] / 16 * (1 + 1e-5), low)).all()
+
+
+def test_norm_on_two_streams_and_of_one_tensor_twice():
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    gs = [[torch.randn(3_000_000, generator=gen, device=DEV)] * 2 for _ in range(2)]
+    want = [MO().grad_norm(g, 1.0).tolist() for g in gs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                outs[k].append(MO().grad_norm(gs[k], 1.0))
+    torch.cuda.synchronize()
+    assert all(o.tolist() == want[k] for k in range(2) for o in outs[k])
+    assert want[0][0] == pytest.approx(math.sqrt(2) * float(gs[0][0].double().norm()), rel=1e-6)
+
+
+def test_captured_norm_and_eviction_replay():
+    gen = torch.Generator(device=DEV).manual_seed(32)
+    for P in (3000, 20_000):
+        s, w, x = torch.rand(P, generator=gen, device=DEV), torch.rand(3, P, generator=gen, device=DEV), torch.randn(P, 3, generator=gen, device=DEV)
+        MO().evict_rows(s, P // 2, [x], weights=w)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = MO().grad_norm([x], 1.0)
+            kept, scores, (y,), _ = MO().evict_rows(s, P // 2, [x], recent=5, weights=w, decay=0.5)
+        for _ in range(4):
+            s.copy_(torch.rand(P, generator=gen, device=DEV)); w.copy_(torch.rand(3, P, generator=gen, device=DEV)); x.copy_(torch.randn(P, 3, generator=gen, device=DEV))
+            graph.replay()
+            torch.cuda.synchronize()
+            k2, s2, (y2,), _ = MO().evict_rows(s, P // 2, [x], recent=5, weights=w, decay=0.5)
+            assert torch.equal(kept, k2) and torch.equal(scores, s2) and torch.equal(y, y2) and torch.equal(norm, MO().grad_norm([x], 1.0))
+
+
+@pytest.mark.parametrize("P", [8192, 8193, 2_200_003])
+def test_evict_tiles_of_more_than_a_pass(P):
+    gen = torch.Generator(device=DEV).manual_seed(33)
+    s = torch.randint(0, 40, (P,), generator=gen, device=DEV).float()
+    x = torch.arange(P, device=DEV)
+    for keep, recent in ((P - 7, 0), (P // 2, 1000), (3, 1)):
+        kept, _, (y,), _ = MO().evict_rows(s, keep, [x], recent=recent)
+        want, _ = O.evict(s.cpu().numpy(), keep, recent)
+        assert np.array_equal(kept.cpu().numpy(), want) and torch.equal(y, kept)
+
+
+def test_evict_codes_past_4_gigabytes():
+    P, width = 1_300_000, 3400
+    rms = torch.empty(P, width, dtype=torch.uint8, device=DEV)
+    rms[:] = (torch.arange(P, device=DEV) % 200 + 30).to(torch.uint8)[:, None]
+    window = torch.full(((P * width + 255) // 256,), 90, dtype=torch.uint8, device=DEV)
+    s = torch.zeros(P, device=DEV)
+    s[P - 700_000:] = 1.0
+    kept, _, (r,), ((c, w),) = MO().evict_rows(s, 700_000, [rms.view(torch.int8)], rms=[(rms, window)])
+    assert kept[0] == P - 700_000 and torch.equal(r[-50:], rms.view(torch.int8)[kept[-50:]]) and torch.equal(r[:50], rms.view(torch.int8)[kept[:50]])
+    # the last 1280 rows begin on a block's border (3400 * 1280 and 700 000 * 3400 are multiples of 256)
+    lo = (700_000 - 1280) * width
+    assert lo % 256 == 0
+    _, (u,) = MO().moments_8bit([c[-1280:].reshape(-1)], [torch.zeros(1280 * width, dtype=torch.int8, device=DEV)], [w[lo // 256:]])
+    assert np.array_equal(n64(u), O.decode(rms[-1280:].cpu().numpy(), np.full(1280 * width // 256, 90)))
+
+
+def test_copies_and_pickles_of_the_optimizer():
+    import copy
+    import pickle
+    gen = torch.Generator(device=DEV).manual_seed(34)
+    ps, opt = small_map(100, gen, 8, max_norm=0.5, seed=77)
+    fill_grads(opt, gen)
+    opt.step()
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.max_norm == 0.5 and other.seed == 77
+        for g, h in zip(opt.param_groups, other.param_groups):
+            for k, v in opt.state[g["params"][0]].items():
+                assert torch.equal(v, other.state[h["params"][0]][k])
+            h["params"][0].grad = torch.ones_like(h["params"][0])
+        other.step()
