@@ -74,6 +74,7 @@ struct NormArgs {
     int count;
     uint32_t chunks;
     double* partial;            // one sum per workgroup
+    float max_norm; float* out; // out: nullable; a launch of one workgroup that writes the result itself
     NormTensor t[GSR_NORM_MAX];
 };
 
@@ -119,6 +120,15 @@ __device__ __forceinline__ void norm_chunk(const NormTensor& t, long long base, 
     }
 }
 
+// torch.nn.utils.clip_grad_norm_'s coefficient: min(1, max_norm / (norm + 1e-6)), a NaN norm stays one.
+__device__ __forceinline__ void norm_out(double sum, float max_norm, float* out)
+{
+    const float norm = (float)sqrt(sum);
+    const float c = max_norm / (norm + 1e-6f);
+    out[0] = norm;
+    out[1] = c > 1.0f ? 1.0f : c;
+}
+
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_grad_norm(NormArgs a)
 {
     __shared__ double s[4];
@@ -132,23 +142,17 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_grad_norm(NormArgs a)
         else norm_chunk<GSR_T_F16>(t, base, sum);
     }
     const double total = opt_block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), s);
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
+    if (threadIdx.x == 0) { if (a.out) norm_out(total, a.max_norm, a.out); else a.partial[blockIdx.x] = total; }
 }
 
-// The partial sums in a fixed order (the result does not depend on which workgroup ran when), then torch.nn.utils.clip_grad_norm_'s
-// coefficient: min(1, max_norm / (norm + 1e-6)), a NaN norm stays one.
+// The partial sums in a fixed order: the result does not depend on which workgroup ran when.
 __global__ void __launch_bounds__(GSR_OPT_THREADS) k_grad_norm_finish(const double* __restrict__ partial, int n, float max_norm, float* __restrict__ out)
 {
     __shared__ double s[4];
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += GSR_OPT_THREADS) sum += partial[i];
     sum = opt_block_sum(sum, s);
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(sum);
-        const float c = max_norm / (norm + 1e-6f);
-        out[0] = norm;
-        out[1] = c > 1.0f ? 1.0f : c;
-    }
+    if (threadIdx.x == 0) norm_out(sum, max_norm, out);
 }
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------------------
