@@ -185,27 +185,23 @@ __device__ __forceinline__ float opt_uniform(float x) { return __uint_as_float(_
 // under their latency), kept in scalar registers.
 //
 // The step counts live on the device, so that a captured graph goes on counting.  They may advance once every workgroup has read them.  A
-// launch of up to GSR_OPT_TICKETS workgroups does it by itself: a workgroup whose waves all have the clock draws a ticket (the fourth
-// word of the launch's first clock, zero between launches), and the one that drew the last advances the clocks when it is done.
-// No fence: nothing but "has read" is handed over (a release at device scope writes the XCD's L2 back, 57 ns per workgroup).  Same-address
-// atomics take turns, 5 ns each whether their workgroup waits or not, so a larger launch leaves it to k_adamw_advance behind it: 34.5 M
-// elements, 8424 workgroups: 302 us with tickets and fences, 209 with tickets, 169 + 4 with the launch.
+// launch of up to GSR_OPT_TICKETS workgroups does it by itself: a workgroup draws a ticket when it is done (the fourth word of the
+// launch's first clock, zero between launches), and the one that drew the last advances the clocks.  No fence: nothing but "has read" is
+// handed over, and what a wave has stored it has computed from the clock (a release at device scope writes the XCD's L2 back, 57 ns
+// per workgroup).  Same-address atomics take turns, 5 ns each, so a larger launch leaves it to k_adamw_advance behind it: 34.5 M
+// elements, 8424 workgroups: 302 us with tickets and fences, 209 with tickets, 167 + 4 with the launch.
 #define GSR_OPT_TICKETS 512
-struct OptRates { float shrink, rate, unbias; uint32_t key, ticket; };
-__device__ __forceinline__ void opt_begin(const OptArgs& a, const OptTensor& t, OptRates& r)          // every wave of a workgroup, once
+struct OptRates { float shrink, rate, unbias; uint32_t key; };
+__device__ __forceinline__ OptRates opt_rates(const OptArgs& a, const OptTensor& t)
 {
     const double lr = t.lr_device ? *t.lr_device : t.lr;
     const double b1t = t.clock[0] * a.beta1, b2t = t.clock[1] * a.beta2;
+    OptRates r;
     r.shrink = opt_uniform((float)(1.0 - lr * t.decay));
     r.rate = opt_uniform((float)((1.0 / (1.0 - b1t)) * lr));
     r.unbias = opt_uniform((float)(1.0 / sqrt(1.0 - b2t)));
     r.key = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t.key + (uint32_t)(t.clock[2] + 1.0)));
-    r.ticket = 0;
-    if (gridDim.x > GSR_OPT_TICKETS) return;
-    // the values, so that the clock has arrived, and not only been asked for, before the barrier
-    asm volatile("" : : "s"(__float_as_uint(r.shrink)), "s"(__float_as_uint(r.rate)), "s"(__float_as_uint(r.unbias)), "s"(r.key) : "memory");
-    __syncthreads();          // all four waves have it
-    if (threadIdx.x == 0) r.ticket = __hip_atomic_fetch_add(reinterpret_cast<unsigned*>(a.t[0].clock + 3), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return r;
 }
 __device__ __forceinline__ void opt_advance(const OptArgs& a)          // one wave
 {
@@ -215,9 +211,14 @@ __device__ __forceinline__ void opt_advance(const OptArgs& a)          // one wa
         if (i == 0) c[3] = 0.0;
     }
 }
-__device__ __forceinline__ void opt_end(const OptArgs& a, const OptRates& r)
+__device__ __forceinline__ void opt_end(const OptArgs& a)          // every wave of the workgroup
 {
-    if (gridDim.x <= GSR_OPT_TICKETS && threadIdx.x < 64 && (uint32_t)__builtin_amdgcn_readfirstlane((int)r.ticket) == gridDim.x - 1u) opt_advance(a);
+    if (gridDim.x > GSR_OPT_TICKETS) return;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    uint32_t ticket = 0;
+    if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(reinterpret_cast<unsigned*>(a.t[0].clock + 3), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if ((uint32_t)__builtin_amdgcn_readfirstlane((int)ticket) == gridDim.x - 1u) opt_advance(a);
 }
 __global__ void __launch_bounds__(64) k_adamw_advance(OptArgs a) { opt_advance(a); }
 
@@ -230,7 +231,7 @@ __device__ __forceinline__ float adamw_one(const OptArgs& a, const OptRates& r, 
 }
 
 template <int PT, int GT, bool STREAM>
-__device__ __forceinline__ void adamw_chunk(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long base)
+__device__ __forceinline__ void adamw_chunk(const OptArgs& a, const OptTensor& t, float coef, long long base)
 {
     float* pm = static_cast<float*>(t.s0);
     float* pv = static_cast<float*>(t.s1);
@@ -243,7 +244,7 @@ __device__ __forceinline__ void adamw_chunk(const OptArgs& a, const OptTensor& t
             m[u] = opt_load4<GSR_T_F32, STREAM>(pm, i); v[u] = opt_load4<GSR_T_F32, STREAM>(pv, i);
         }
     }
-    opt_begin(a, t, r);
+    const OptRates r = opt_rates(a, t);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
         const long long i = base + 4 * (u * GSR_OPT_THREADS + (int)threadIdx.x);
@@ -262,12 +263,12 @@ __device__ __forceinline__ void adamw_chunk(const OptArgs& a, const OptTensor& t
 }
 
 // Pointers that are not aligned to four elements: one element per lane and load, any types.
-__device__ __forceinline__ void adamw_chunk_unaligned(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long base)
+__device__ __forceinline__ void adamw_chunk_unaligned(const OptArgs& a, const OptTensor& t, float coef, long long base)
 {
     float* pm = static_cast<float*>(t.s0);
     float* pv = static_cast<float*>(t.s1);
     const int pt = t.types & 15, gt = (t.types >> 4) & 15;
-    opt_begin(a, t, r);
+    const OptRates r = opt_rates(a, t);
     for (int k = threadIdx.x; k < GSR_OPT_CHUNK && base + k < t.n; k += GSR_OPT_THREADS) {
         const long long j = base + k;
         opt_store(t.p, j, pt, adamw_one(a, r, coef, opt_load(t.p, j, pt), opt_load(t.g, j, gt), pm[j], pv[j]));
@@ -279,15 +280,14 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw(OptArgs a)
 {
     const float coef = a.clip ? a.clip[1] : 1.0f;
     const OptTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];          // (of no elements at all: a launch of one workgroup that advances the clocks)
-    OptRates r;
     const long long base = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK;
     switch (t.types) {
-#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw_chunk<P, G, STREAM>(a, t, r, coef, base); break;
+#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw_chunk<P, G, STREAM>(a, t, coef, base); break;
     GSR_OPT_CASE(0, 0) GSR_OPT_CASE(0, 1) GSR_OPT_CASE(0, 2) GSR_OPT_CASE(1, 0) GSR_OPT_CASE(1, 1) GSR_OPT_CASE(1, 2) GSR_OPT_CASE(2, 0) GSR_OPT_CASE(2, 1) GSR_OPT_CASE(2, 2)
 #undef GSR_OPT_CASE
-    default: adamw_chunk_unaligned(a, t, r, coef, base);
+    default: adamw_chunk_unaligned(a, t, coef, base);
     }
-    opt_end(a, r);
+    opt_end(a);
 }
 
 // ---- AdamW with a byte for each moment -------------------------------------------------------------------------------------------
@@ -355,10 +355,11 @@ __device__ __forceinline__ void opt_sqrt4(const float (&x)[4], float (&s)[4])
     }
 }
 
-// One wave, four blocks of 256 from `start`, all loads in flight together (two of them: 143 us for 132 over 47 M elements): four consecutive elements per lane.  FULL: every block lies inside the tensor and all
-// pointers are aligned (PT, GT: the types); otherwise element by element, any types.
+// One wave, four blocks of 256 from `start`, four consecutive elements per lane, all loads in flight together (of two blocks: 143 us for 132
+// over 47 M elements).  FULL: every block lies inside the tensor and all pointers are aligned (PT, GT: the types); otherwise element by
+// element, any types.
 template <int PT, int GT, bool FULL, bool STREAM>
-__device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor& t, OptRates& r, float coef, long long start)
+__device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor& t, float coef, long long start)
 {
     const int pt = FULL ? PT : t.types & 15, gt = FULL ? GT : (t.types >> 4) & 15;
     const int lane = threadIdx.x & 63;
@@ -384,7 +385,7 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
                 }
         }
     }
-    opt_begin(a, t, r);
+    const OptRates r = opt_rates(a, t);
     const uint32_t key = opt_mix(r.key);
 #pragma unroll
     for (int b = 0; b < 4; b++) {
@@ -450,20 +451,17 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw8(OptArgs a)
 {
     const float coef = a.clip ? a.clip[1] : 1.0f;
     const OptTensor& t = a.t[opt_find(a.t, a.count, blockIdx.x)];
-    OptRates r;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const long long start = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK + wave * (GSR_OPT_CHUNK / 4);
     if (start < t.n) {
         switch (start + GSR_OPT_CHUNK / 4 <= t.n ? t.types : 0) {
-#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw8_blocks<P, G, true, STREAM>(a, t, r, coef, start); break;
+#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw8_blocks<P, G, true, STREAM>(a, t, coef, start); break;
         GSR_OPT_CASE(0, 0) GSR_OPT_CASE(0, 1) GSR_OPT_CASE(0, 2) GSR_OPT_CASE(1, 0) GSR_OPT_CASE(1, 1) GSR_OPT_CASE(1, 2) GSR_OPT_CASE(2, 0) GSR_OPT_CASE(2, 1) GSR_OPT_CASE(2, 2)
 #undef GSR_OPT_CASE
-        default: adamw8_blocks<0, 0, false, false>(a, t, r, coef, start);
+        default: adamw8_blocks<0, 0, false, false>(a, t, coef, start);
         }
-    } else {
-        opt_begin(a, t, r);          // (to the other waves' barrier)
     }
-    opt_end(a, r);
+    opt_end(a);
 }
 
 struct MomentTensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg; void* root; long long n; uint32_t first; int aligned; };
@@ -545,7 +543,8 @@ struct EvictArgs {
 };
 
 // The accumulated weights of U rows, summed in the views' order.  No load waits for another: rows behind the end load the last row again,
-// views behind the last the last view (a load under a condition is waited for where it stands: k_evict_scores 22 us at 1.5 M rows and 4 views, 15 so).
+// views behind the last the last view (a load under a condition is waited for where it stands: k_evict_scores 22 us at 1.5 M rows and 4
+// views, 15 so).
 template <int U>
 __device__ __forceinline__ void evict_scores(const EvictArgs& a, const long long (&i)[U], float (&s)[U])
 {
