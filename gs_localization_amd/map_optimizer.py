@@ -232,26 +232,34 @@ def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=())
         if weights.dtype is not torch.float32 or weights.dim() != 2 or weights.shape[1] != P:
             raise ValueError("evict_rows: weights is float32 [views, P] or [P]")
     scores = scores.contiguous()
-    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    rms = [(c if c.is_contiguous() else c.contiguous(), w if w.is_contiguous() else w.contiguous()) for c, w in rms]
-    index = _device([scores] + ([] if weights is None else [weights]) + tensors + [x for pair in rms for x in pair], "evict_rows")
-    n = len(tensors) + len(rms)
-    buf, rows, pairs = bytearray(_ROW.size * n), [], []
+    index = _device([scores, *(() if weights is None else (weights,)), *tensors, *[x for pair in rms for x in pair]], "evict_rows")
+    n, size = len(tensors) + len(rms), _ROW.size
+    buf, rows, pairs, held = bytearray(size * n), [], [], []
     with _on(index) as stream:
         out = scores.new_empty(keep)
         kept = torch.empty(keep, dtype=torch.int64, device=scores.device)
-        for i, t in enumerate(tensors):
-            if t.dim() < 1 or t.shape[0] != P:
-                raise ValueError(f"evict_rows: tensor {i} has shape {tuple(t.shape)}, {P} rows wanted")
-            y = t.new_empty((keep, *t.shape[1:]))
+        at = 0
+        for t in tensors:
+            shape = t.shape
+            if not shape or shape[0] != P:
+                raise ValueError(f"evict_rows: tensor {len(rows)} has shape {tuple(shape)}, {P} rows wanted")
+            if not t.is_contiguous():
+                t = t.contiguous()
+                held.append(t)
+            y = t.new_empty((keep, *shape[1:]))
             rows.append(y)
-            _ROW.pack_into(buf, _ROW.size * i, t.data_ptr(), y.data_ptr(), 0, 0, t.element_size() * (t.numel() // P) if P else 0)
-        for i, (c, w) in enumerate(rms):
-            if c.dim() < 1 or c.shape[0] != P or c.dtype is not torch.uint8 or w.dtype is not torch.uint8 or w.numel() != (c.numel() + WINDOW - 1) // WINDOW:
-                raise ValueError(f"evict_rows: rms {i}: codes uint8 [P, ...] and their window uint8 required")
-            row = c.numel() // P if P else 0
+            _ROW.pack_into(buf, at, t.data_ptr(), y.data_ptr(), 0, 0, t.nbytes // P if P else 0)
+            at += size
+        for c, w in rms:
+            k = c.numel()
+            if c.dim() < 1 or c.shape[0] != P or c.dtype is not torch.uint8 or w.dtype is not torch.uint8 or w.numel() != (k + WINDOW - 1) // WINDOW:
+                raise ValueError(f"evict_rows: rms {len(pairs)}: codes uint8 [P, ...] and their window uint8 required")
+            c, w = c.contiguous(), w.contiguous()
+            held += (c, w)
+            row = k // P if P else 0
             pairs.append((c.new_empty((keep, *c.shape[1:])), w.new_empty((keep * row + WINDOW - 1) // WINDOW)))
-            _ROW.pack_into(buf, _ROW.size * (len(tensors) + i), c.data_ptr(), pairs[i][0].data_ptr(), w.data_ptr(), pairs[i][1].data_ptr(), row)
+            _ROW.pack_into(buf, at, c.data_ptr(), pairs[-1][0].data_ptr(), w.data_ptr(), pairs[-1][1].data_ptr(), row)
+            at += size
         ws_t, ws = _workspace(lib.gsr_evict_bytes(P), index)
         args = _lib.EvictArgs(P, 0 if weights is None else weights.shape[0], keep, recent, scores.data_ptr(),
                               None if weights is None else weights.data_ptr(), decay, kept.data_ptr(), out.data_ptr(), n, _address(buf),
