@@ -355,20 +355,31 @@ __device__ __forceinline__ void opt_sqrt4(const float (&x)[4], float (&s)[4])
     }
 }
 
-// One wave, four blocks of 256 from `start`, four consecutive elements per lane, all loads in flight together (of two blocks: 143 us for 132
-// over 47 M elements).  FULL: every block lies inside the tensor and all pointers are aligned (PT, GT: the types); otherwise element by
-// element, any types.
-template <int PT, int GT, bool FULL, bool STREAM>
+// a / b for b in [2^-100, 2^100], by a refined reciprocal and one residual (Markstein's scheme: the quotient is the correctly rounded one but
+// for residuals that underflow, of |a| under 2^-100).  The division operator spends five more instructions on scaling for any b; roots are
+// in [2^-75, 2^64] here, squares of floats having been under them.
+__device__ __forceinline__ float opt_div(float a, float b)
+{
+    float r = __builtin_amdgcn_rcpf(b);
+    r = __builtin_fmaf(__builtin_fmaf(-b, r, 1.0f), r, r);
+    const float q = a * r;
+    return __builtin_fmaf(__builtin_fmaf(-b, q, a), r, q);
+}
+
+// One wave, NB blocks of 256 from `start`, four consecutive elements per lane, all loads in flight together.  FULL: every block lies inside the
+// tensor and all pointers are aligned (PT, GT: the types), four blocks (two: 143 us for 132 over 47 M elements); otherwise element by
+// element, any types, one block (four need 195 registers, which the whole kernel then has: 162 us for 128).
+template <int PT, int GT, bool FULL, bool STREAM, int NB>
 __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor& t, float coef, long long start)
 {
     const int pt = FULL ? PT : t.types & 15, gt = FULL ? GT : (t.types >> 4) & 15;
     const int lane = threadIdx.x & 63;
     uint8_t* rms = static_cast<uint8_t*>(t.s0);
     int8_t* ratio = static_cast<int8_t*>(t.s1);
-    opt_f4 p[4], g[4];
-    uint32_t cu[4], cr[4], old[4];
+    opt_f4 p[NB], g[NB];
+    uint32_t cu[NB], cr[NB], old[NB];
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
+    for (int b = 0; b < NB; b++) {
         const long long s = start + b * GSR_OPT_WINDOW, i = s + 4 * lane;
         p[b] = 0.0f; g[b] = 0.0f; cu[b] = cr[b] = old[b] = 0u;
         if (FULL) {
@@ -386,9 +397,9 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
         }
     }
     const OptRates r = opt_rates(a, t);
-    const uint32_t key = opt_mix(r.key);
+    const uint32_t key = opt_mix(r.key), lane_mul = (uint32_t)lane * 0x9E3779B1u;
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
+    for (int b = 0; b < NB; b++) {
         const long long s = start + b * GSR_OPT_WINDOW, i = s + 4 * lane;
         if (!FULL && s >= t.n) break;          // (the whole wave)
         const uint32_t was = 16u * old[b] + 1u;
@@ -403,24 +414,25 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
         opt_sqrt4(v1, u1);
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            p[b][k] = p[b][k] * r.shrink - (m1[k] / (u1[k] * r.unbias + a.eps)) * r.rate;
-            top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
-        }
+        for (int k = 0; k < 4; k++) top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
         top = wave_max_u32(top);
-        if (top >= 0x7f800000u) {          // an infinite root or a NaN (the whole wave comes here, or none): its neighbours' window is that of the finite ones
+        if (top >= 0x7f800000u || a.eps < 0x1p-100f) {          // an infinite root or a NaN (the whole wave comes here, or none), or roots of 0 over next to nothing
             top = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                if (__float_as_uint(u1[k]) >= 0x7f800000u) u1[k] = __builtin_inff();          // -> code 255
+                p[b][k] = p[b][k] * r.shrink - (m1[k] / (u1[k] * r.unbias + a.eps)) * r.rate;
+                if (__float_as_uint(u1[k]) >= 0x7f800000u) u1[k] = __builtin_inff();          // -> code 255; its neighbours' window is that of the finite ones
                 else top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
                 if (m1[k] != m1[k]) m1[k] = 0.0f;
             }
             top = wave_max_u32(top);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) p[b][k] = p[b][k] * r.shrink - opt_div(m1[k], u1[k] * r.unbias + a.eps) * r.rate;
         }
         const uint32_t w = opt_window(top), now = 16u * w + 1u;
         // (the upper half of the quad's number is the whole block's)
-        const uint32_t h = opt_mix(((((uint32_t)(s >> 2) + lane) * 0x9E3779B1u) ^ key) + (uint32_t)(s >> 34) * 0x85EBCA77u);
+        const uint32_t h = opt_mix((((uint32_t)(s >> 2) * 0x9E3779B1u + lane_mul) ^ key) + (uint32_t)(s >> 34) * 0x85EBCA77u);
         uint32_t nu = 0, nr = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -428,12 +440,14 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
             int code = (int)((bits + (d >> 13)) >> 19) - (int)now;
             code = code < 1 ? 1 : (code > 255 ? 255 : code);
             code = bits == 0u ? 0 : code;
-            const float u = __uint_as_float(((uint32_t)code + now) << 19);          // (of a code 0: some number > 0, the quotient is not used)
-            const float q = floorf((m1[k] / u) * a.per_unit + (float)(d & 8191u) * (1.0f / 8192.0f));
-            const int n = bits == 0u ? 0 : (int)__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f);
+            const float u = __uint_as_float(((uint32_t)code + now) << 19);          // (of a code 0: some number, the quotient is not used)
+            // (the random bits times 2^-13 are exact: one rounding, as of a sum)
+            float q = floorf(__builtin_fmaf((float)(d & 8191u), 1.0f / 8192.0f, opt_div(m1[k], u) * a.per_unit));
+            q = bits == 0u ? 0.0f : __builtin_amdgcn_fmed3f(q, -127.0f, 127.0f);
             nu |= (uint32_t)code << (8 * k);
-            nr |= ((uint32_t)n & 255u) << (8 * k);
+            nr = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.0f, k, nr);          // a whole number in 1 ... 255 into byte k
         }
+        nr ^= 0x80808080u;          // less 128: two's complement
         if (FULL) {
             opt_store4<PT, STREAM>(t.p, i, p[b]);
             opt_put<STREAM>(reinterpret_cast<uint32_t*>(rms + i), nu); opt_put<STREAM>(reinterpret_cast<uint32_t*>(ratio + i), nr);
@@ -455,10 +469,13 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw8(OptArgs a)
     const long long start = (long long)(blockIdx.x - t.first) * GSR_OPT_CHUNK + wave * (GSR_OPT_CHUNK / 4);
     if (start < t.n) {
         switch (start + GSR_OPT_CHUNK / 4 <= t.n ? t.types : 0) {
-#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw8_blocks<P, G, true, STREAM>(a, t, coef, start); break;
+#define GSR_OPT_CASE(P, G) case P | G << 4 | GSR_T_ALIGNED: adamw8_blocks<P, G, true, STREAM, 4>(a, t, coef, start); break;
         GSR_OPT_CASE(0, 0) GSR_OPT_CASE(0, 1) GSR_OPT_CASE(0, 2) GSR_OPT_CASE(1, 0) GSR_OPT_CASE(1, 1) GSR_OPT_CASE(1, 2) GSR_OPT_CASE(2, 0) GSR_OPT_CASE(2, 1) GSR_OPT_CASE(2, 2)
 #undef GSR_OPT_CASE
-        default: adamw8_blocks<0, 0, false, false>(a, t, coef, start);
+        default:
+#pragma unroll 1
+            for (int b = 0; b < 4; b++)
+                if (start + b * GSR_OPT_WINDOW < t.n) adamw8_blocks<0, 0, false, false, 1>(a, t, coef, start + b * GSR_OPT_WINDOW);
         }
     }
     opt_end(a);
