@@ -867,3 +867,96 @@ def test_copies_and_pickles_of_the_optimizer():
                 assert torch.equal(v, other.state[h["params"][0]][k])
             h["params"][0].grad = torch.ones_like(h["params"][0])
         other.step()
+
+
+# ---- what the documentation allows and nothing above does -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-15, 1e-40, 0.0])
+def test_first_8_bit_step_is_the_32_bit_one(eps):
+    """From zero moments nothing is rounded to a byte before the parameter is stepped: the same bits as with 32-bit moments, so the 8-bit kernel's own
+    square root and quotient are the correctly rounded ones.  Gradients of every binade whose square and moments are normal floats, some zero."""
+    n = 1 << 22
+    gen = torch.Generator(device=DEV).manual_seed(40)
+    g = torch.randn(n, generator=gen, device=DEV) * torch.exp2(torch.randint(-55, 60, (n,), generator=gen, device=DEV).float())
+    g *= torch.rand(n, generator=gen, device=DEV) < 0.9
+    p0 = torch.randn(n, generator=gen, device=DEV)
+    p, q = p0.clone(), p0.clone()
+    rms, ratio, window = torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.int8, device=DEV), torch.zeros(n // 256, dtype=torch.uint8, device=DEV)
+    MO().adamw_step([p], [g], [torch.zeros_like(p)], [torch.zeros_like(p)], clocks(1, 0, (0.9, 0.999)), lr=0.37, eps=eps, weight_decay=0.1)
+    MO().adamw_step_8bit([q], [g], [rms], [ratio], [window], clocks(1, 0, (0.9, 0.999)), lr=0.37, eps=eps, weight_decay=0.1)
+    assert torch.equal(p.view(torch.int32)[g != 0], q.view(torch.int32)[g != 0])
+    if eps:
+        assert torch.equal(p[g == 0], q[g == 0]) and bool(q.isfinite().all())
+    else:          # (0 / 0, as torch)
+        assert bool(p[g == 0].isnan().all()) and bool(q[g == 0].isnan().all())
+
+
+def test_groups_of_both_kinds_clip_together():
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    a, b, c = (torch.nn.Parameter(torch.randn(n, generator=gen, device=DEV)) for n in (100, 3000, 7))
+    opt = MO().AdamW([{"params": [a], "lr": 0.1}, {"params": [b], "lr": 0.2, "state_bits": 8}, {"params": [c], "betas": (0.5, 0.9), "eps": 1e-3, "weight_decay": 0.1}], max_norm=0.3)
+    for t in (1, 2):
+        before = [x.detach().clone() for x in (a, b, c)]
+        state = {x: {k: v.clone() for k, v in opt.state[x].items()} for x in (a, c) if x in opt.state}
+        for x in (a, b, c):
+            x.grad = torch.randn(x.shape, generator=gen, device=DEV)
+        seen = []
+        loss = opt.step(lambda: seen.append(torch.is_grad_enabled()) or torch.tensor(3.0))
+        assert float(loss) == 3.0 and seen == [True]
+        n, coef = O.norm([n64(x.grad) for x in (a, b, c)], 0.3)
+        assert abs(float(opt.last_norm[0]) - n) <= 2 * E * n
+        coef = float(opt.last_norm[1])
+        for x, old, lr, betas, eps, wd in ((a, before[0], 0.1, (0.9, 0.999), 1e-8, 0.0), (c, before[2], 1e-3, (0.5, 0.9), 1e-3, 0.1)):
+            m, v = (n64(state[x][k]) for k in ("exp_avg", "exp_avg_sq")) if x in state else (0, 0)
+            p1, m1, v1, scale = O.adamw(n64(old), n64(x.grad), m, v, t, lr, betas, eps, wd, coef)
+            assert (np.abs(n64(x) - p1) <= bound32(p1, m1, v1, scale, lr, wd, torch.float32)).all()
+        assert set(opt.state[b]) == {"rms", "ratio", "window", "step"}
+    # eviction where only some have moments: c's rows are not the others', so it is refused and nothing has changed
+    kept = [x.detach().clone() for x in (a, b, c)]
+    with pytest.raises(ValueError, match="rows"):
+        opt.evict(torch.rand(100, device=DEV), 50)
+    assert all(torch.equal(x, y) for x, y in zip(kept, (a, b, c))) and opt.param_groups[0]["params"][0] is a
+
+
+def test_scheduler_sets_the_rate():
+    p = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    opt = MO().AdamW([p], lr=1.0)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+    total = 0.0
+    for k in range(4):
+        p.grad = torch.ones_like(p)
+        opt.step()
+        sched.step()
+        total += 0.5 ** k
+    # equal gradients: every step is the rate, to the roundings of the moments (some 10 e each)
+    assert float((p.detach() + total).abs().max()) < 4 * 20 * E * 2
+
+
+def test_evict_takes_any_layout():
+    P = 5000
+    gen = torch.Generator(device=DEV).manual_seed(42)
+    s = torch.rand(P, 2, generator=gen, device=DEV)[:, 0]
+    w = torch.rand(P, generator=gen, device=DEV)
+    p = torch.nn.Parameter(torch.randn(P, 3, generator=gen, device=DEV))
+    d = torch.randn(P, 2, generator=gen, device=DEV, dtype=torch.float64)
+    rms = torch.randint(0, 255, (3, P), generator=gen, device=DEV).to(torch.uint8).t()
+    window = torch.full((2 * ((P * 3 + 255) // 256),), 100, dtype=torch.uint8, device=DEV)[::2]
+    kept, scores, (q, e), ((c, cw),) = MO().evict_rows(s, 2000, [p, d], weights=w, rms=[(rms, window)])
+    want, ws = O.evict(s.cpu().numpy(), 2000, 0, w.cpu().numpy()[None])
+    assert np.array_equal(kept.cpu().numpy(), want) and np.array_equal(scores.cpu().numpy(), ws)
+    assert torch.equal(q, p.detach()[kept]) and not q.requires_grad and torch.equal(e, d[kept])
+    u = O.decode(rms.contiguous().cpu().numpy(), np.full((P * 3 + 255) // 256, 100)).reshape(P, 3)[want].reshape(-1)
+    assert np.array_equal(O.decode(c.cpu().numpy(), cw.cpu().numpy()), np.where(u > 0, np.maximum(u, O.grid_value(16 * O.per_block(cw.cpu().numpy(), u.size) + 2)), 0))
+    for bad in (dict(tensors=[d[:10]]), dict(tensors=[torch.tensor(1.0, device=DEV)]), dict(tensors=[], rms=[(rms, window[:3])]), dict(tensors=[], weights=w[:5])):
+        with pytest.raises(ValueError):
+            MO().evict_rows(s, 2000, **bad)
+    with pytest.raises(RuntimeError, match="HIP tensors"):
+        MO().evict_rows(s, 2000, [torch.zeros(P)])
+
+
+def test_sparse_gradient_is_refused():
+    emb = torch.nn.Embedding(10, 4, sparse=True, device=DEV)
+    opt = MO().AdamW(emb.parameters())
+    emb(torch.tensor([1, 2], device=DEV)).sum().backward()
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()

@@ -194,7 +194,7 @@ def test_evict_c_refusals():
         return lib.gsr_evict_rows(C.byref(_lib.EvictArgs(*a.values()))), lib.gsr_last_error().decode()
     for kw, what in ((dict(P=-1, keep=0), "negative"), (dict(keep=9), "recent <= keep <= P"), (dict(recent=5), "recent <= keep <= P"), (dict(n_views=-1), "negative"),
                      (dict(n_views=1), "NULL"), (dict(scores=None), "NULL"), (dict(kept=None), "NULL"), (dict(tensors=None), "NULL"),
-                     (dict(row=(0, 0x20000, 0, 0, 12)), "NULL"), (dict(row=(0x10000, 0x20000, 0x30000, 0, 12)), "NULL"), (dict(row=(0x10000, 0x20000, 0, 0, -1)), "row size"),
+                     (dict(row=(0, 0x20000, 0, 0, 12)), "NULL"), (dict(row=(0x10000, 0x20000, 0x30000, 0, 12)), "NULL"), (dict(row=(0x10000, 0x20000, 0, 0, -1)), "row size"), (dict(row=(0x10000, 0x20000, 0, 0, 1 << 31)), "row size"), (dict(P=1 << 30, row=(0x10000, 0x20000, 0, 0, 1 << 10)), "row size"),
                      (dict(row=(0x10000, 0x10020, 0, 0, 12)), "overlaps"), (dict(scores_out=0x2010), "overlaps"), (dict(kept=0x1008), "overlaps")):
         rc, said = call(**kw)
         assert rc == -1 and what in said, (kw, rc, said)
