@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
 // the rows' places by counting per tile of rows; every tensor of the map and of its optimiser is then compacted in one launch.  No
 // workgroup ever waits for another: a launch's end is the only barrier between them.
 
-#define GSR_EV_UNITS 16         // units of a lane whose loads are in flight together (4: 178 us for 1.35 M rows of 281 bytes, 8: 173, 16: 154)
+#define GSR_EV_UNITS 16         // units of a lane whose loads are in flight together (4: 178 us for 1.35 M rows of 281 bytes, 8: 173, 16: 159; 32 of twice as large a chunk: 171)
 #define GSR_EV_BLOCKS 4         // blocks of codes likewise
 #define GSR_EV_CHUNK 8192       // units of one byte that a workgroup copies (of others GSR_OPT_CHUNK)
 #define GSR_EV_BINS 2048
@@ -909,13 +909,13 @@ struct RowWalk {
 };
 
 // Consecutive lanes, consecutive units, GSR_EV_UNITS of a lane in flight; nothing is loaded under a condition, which would have each load
-// waited for where it stands (250 us for 1.35 M rows of 281 bytes, 154 so: 776 MB at 5.0 TB/s).  Staging the source's span in LDS, evicted
+// waited for where it stands (250 us for 1.35 M rows of 281 bytes, 159 so: 776 MB at 4.9 TB/s).  Staging the source's span in LDS, evicted
 // rows with it, was slower (280), a workgroup per 256 rows of all tensors as well (166).
 template <class T>
 __device__ __forceinline__ void evict_chunk(const RowArgs& a, const RowTensor& t, long long base, uint32_t chunk)
 {
     constexpr int U = sizeof(T) <= 4 ? GSR_EV_UNITS : GSR_EV_UNITS * 4 / (int)sizeof(T);          // the same bytes, and registers, for every unit
-    typedef unsigned long long OFF;          // (no register is scarce here: 32 bits gain nothing, 160 us for 154)
+    typedef unsigned long long OFF;          // (no register is scarce here: 32 bits gain nothing)
     const RowWalk<OFF> w(a, t, base, chunk);
     const char* src = static_cast<const char*>(t.src);
     T* dst = static_cast<T*>(t.dst) + base;
