@@ -379,8 +379,8 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"load_state_dict: a group with {b}-bit moments got the state {sorted(state_dict['state'][i])}")
         super().load_state_dict(state_dict)
         for b, g, old in zip(bits, self.param_groups, given):
-            for k in set(g) - {"params", "name", "state_bits", *self.defaults} - set(own[0]):
-                del g[k]          # (torch's own options: capturable, foreach, ...)
+            for k in ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"):
+                g.pop(k, None)          # (torch.optim.Adam's own options)
             g["state_bits"] = b
             for i, p in zip(old["params"], g["params"]):
                 if i not in state_dict["state"]:

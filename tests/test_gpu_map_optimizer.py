@@ -928,6 +928,9 @@ def test_scheduler_sets_the_rate():
         opt.step()
         sched.step()
         total += 0.5 ** k
+    again = MO().AdamW([torch.nn.Parameter(p.detach().clone())], lr=1.0)
+    again.load_state_dict(opt.state_dict())
+    assert torch.optim.lr_scheduler.LambdaLR(again, lambda k: 0.5 ** k, last_epoch=3).get_last_lr() == sched.get_last_lr()          # ("initial_lr" came along)
     # equal gradients: every step is the rate, to the roundings of the moments (some 10 e each)
     assert float((p.detach() + total).abs().max()) < 4 * 20 * E * 2
 
