@@ -213,7 +213,7 @@ def moments_8bit(rms, ratio, window, betas=(0.9, 0.999), dtype=torch.float32):
 def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=()):
     """Compacts a map to `keep` of its P rows by accumulated compositing weight.
 
-    scores: float32 [P], accumulated so far; weights: float32 [views, P] or [P], this round's (compositing_weights), or None:
+    scores: float32 [P], accumulated so far; weights: float32 [views, P] or [P], the new views' (compositing_weights), or None:
     score = decay * score + sum of weights.  The last `recent` rows stay whatever their score, and of the others the keep - recent with
     the largest (ties: the lower index; NaN counts as -inf).  tensors: [P, ...] each, of any types; rms: pairs (codes uint8 [P, ...], window)
     of 8-bit moments, re-coded for their new blocks -- exact, but for a root under its new window's sixteen binades, which
