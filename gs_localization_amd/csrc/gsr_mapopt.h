@@ -416,7 +416,8 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
 #pragma unroll
         for (int k = 0; k < 4; k++) top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
         top = wave_max_u32(top);
-        if (top >= 0x7f800000u || a.eps < 0x1p-100f) {          // an infinite root or a NaN (the whole wave comes here, or none), or roots of 0 over next to nothing
+        const bool rare = top >= 0x7f800000u || a.eps < 0x1p-100f;          // an infinite root or a NaN (the whole wave, or none), or roots of 0 over next to nothing
+        if (rare) {
             top = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -441,8 +442,10 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
             code = code < 1 ? 1 : (code > 255 ? 255 : code);
             code = bits == 0u ? 0 : code;
             const float u = __uint_as_float(((uint32_t)code + now) << 19);          // (of a code 0: some number, the quotient is not used)
+            // An overflowed root's momentum may be infinite, or too large for opt_div over what code 255 stands for (2^-111 in a block of nothing else).
+            const float over = rare ? m1[k] / u : opt_div(m1[k], u);
             // (the random bits times 2^-13 are exact: one rounding, as of a sum)
-            float q = floorf(__builtin_fmaf((float)(d & 8191u), 1.0f / 8192.0f, opt_div(m1[k], u) * a.per_unit));
+            float q = floorf(__builtin_fmaf((float)(d & 8191u), 1.0f / 8192.0f, over * a.per_unit));
             q = bits == 0u ? 0.0f : __builtin_amdgcn_fmed3f(q, -127.0f, 127.0f);
             nu |= (uint32_t)code << (8 * k);
             nr = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.0f, k, nr);          // a whole number in 1 ... 255 into byte k
