@@ -416,7 +416,8 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
 #pragma unroll
         for (int k = 0; k < 4; k++) top = __float_as_uint(u1[k]) > top ? __float_as_uint(u1[k]) : top;
         top = wave_max_u32(top);
-        const bool rare = top >= 0x7f800000u || a.eps < 0x1p-100f;          // an infinite root or a NaN (the whole wave, or none), or roots of 0 over next to nothing
+        // An infinite root or a NaN (the whole wave, or none), roots of 0 over next to nothing, a divisor past opt_div's range.
+        const bool rare = top >= 0x7f800000u || a.eps < 0x1p-100f || a.eps > 0x1p99f;
         if (rare) {
             top = 0;
 #pragma unroll

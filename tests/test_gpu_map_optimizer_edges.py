@@ -56,3 +56,17 @@ def test_overflowed_root_keeps_the_momentums_sign(dtype, shift, beside):
     q = torch.ones(n, device=DEV)
     MO().adamw_step_8bit([q], [torch.zeros(n, device=DEV)], [rms1], [ratio1], [window1], clocks(1, 1, (0.9, 0.999)), lr=0.1, seed=3)
     assert ((q[at] - 1.0) * sign <= 0).all()
+
+
+@pytest.mark.parametrize("eps", [1e30, 2.0 ** 100, 1e35, 2.0 ** 127, 3e38, math.inf])
+def test_first_8_bit_step_with_a_large_eps(eps):
+    """The same bits as with 32-bit moments (nothing has been rounded to a byte yet), whatever eps is added to the root."""
+    n = 4096
+    gen = torch.Generator(device=DEV).manual_seed(51)
+    g = torch.randn(n, generator=gen, device=DEV) * torch.exp2(torch.randint(-55, 60, (n,), generator=gen, device=DEV).float())
+    p = torch.randn(n, generator=gen, device=DEV)
+    q = p.clone()
+    a = codes(n)
+    MO().adamw_step([p], [g], [torch.zeros_like(p)], [torch.zeros_like(p)], clocks(1, 0, (0.9, 0.999)), lr=1e25, eps=eps)
+    MO().adamw_step_8bit([q], [g], [a[0]], [a[1]], [a[2]], clocks(1, 0, (0.9, 0.999)), lr=1e25, eps=eps)
+    assert bool(p.isfinite().all()) and torch.equal(p.view(torch.int32), q.view(torch.int32))
