@@ -2076,10 +2076,12 @@ int gsr_grad_norm(int n_tensors, const void* const* grads, const long long* nume
     return no_throw([&] { return grad_norm(n_tensors, grads, numels, types, max_norm, out, workspace, workspace_ctx, stream); });
 }
 
-int gsr_adamw_step(const gsr_adamw_args* args)
+int gsr_adamw_step(const gsr_adamw_args* args) { return gsr_adamw_step_coded(args, nullptr); }
+
+int gsr_adamw_step_coded(const gsr_adamw_args* args, const gsr_code_origin* origins)
 {
     if (!args) return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
-    return no_throw([&] { return adamw_step(args); });
+    return no_throw([&] { return adamw_step(args, origins); });
 }
 
 int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream)

@@ -169,12 +169,13 @@ struct OptTensor {
     uint32_t first;             // its first workgroup in the launch
     uint32_t key;               // 8 bits: seed and place in the list
     int types;                  // parameter | gradient << 4 | GSR_T_ALIGNED
+    float unit;                 // 8 bits: the step of the ratios that it comes with (of the betas they were stored with)
 };
 struct OptArgs {
     int count;
     double beta1, beta2;
     float b1, b2, c1, c2, eps;  // (c = 1 - beta)
-    float unit, per_unit;       // 8 bits: the ratio's step, and steps per one
+    float per_unit;             // 8 bits: steps of the ratio per one, as this step stores it
     const float* clip;          // nullable: (norm, coefficient)
     OptTensor t[GSR_OPT_MAX];
 };
@@ -301,7 +302,8 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw(OptArgs a)
 //   r   |m| <= B sqrt(v) whatever the gradients were, B = (1 - b1) / sqrt((1 - b2)(1 - b1^2 / b2)) (Cauchy-Schwarz over the two
 //       exponential sums; 7.27 for 0.9 / 0.999): 127 steps of B / 127 to either side, stochastic (13 bits).  A momentum quantised for
 //       itself could meet a root that its own block has rounded to almost nothing, and with train.py's eps = 1e-15 the quotient would
-//       throw the splat across the scene; the ratio is the update, and cannot.
+//       throw the splat across the scene; the ratio is the update, and cannot.  (B is that of the step which stores it; where a schedule
+//       changes the betas, a momentum past it is stored as B.)
 // The parameter is stepped with the moments before they are rounded.
 
 __device__ __forceinline__ uint32_t opt_mix(uint32_t x)          // two rounds of xor-shift and odd multiplier (a bijection of 32 bits)
@@ -408,7 +410,7 @@ __device__ __forceinline__ void adamw8_blocks(const OptArgs& a, const OptTensor&
         for (int k = 0; k < 4; k++) {
             const float u = opt_decode((cu[b] >> (8 * k)) & 255u, was);
             const float x = g[b][k] * coef;
-            m1[k] = (((float)(int8_t)(cr[b] >> (8 * k)) * a.unit) * u) * a.b1 + x * a.c1;
+            m1[k] = (((float)(int8_t)(cr[b] >> (8 * k)) * t.unit) * u) * a.b1 + x * a.c1;
             v1[k] = (u * u) * a.b2 + (x * x) * a.c2;
         }
         opt_sqrt4(v1, u1);

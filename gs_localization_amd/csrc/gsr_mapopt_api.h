@@ -34,7 +34,11 @@ struct OptRanges {
     }
 };
 
-int adamw_step(const gsr_adamw_args* a)
+// The largest |m| / sqrt(v) that gradients can bring about: the 8-bit ratio has 127 steps of it to either side.
+bool opt_spannable(double beta1, double beta2) { return beta1 >= 0.0 && beta1 * beta1 < beta2 && beta2 < 1.0; }
+double opt_span(double beta1, double beta2) { return (1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)); }
+
+int adamw_step(const gsr_adamw_args* a, const gsr_code_origin* origins)
 {
     using namespace gsr;
     const int debug = 0;
@@ -44,7 +48,7 @@ int adamw_step(const gsr_adamw_args* a)
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: 0 <= beta < 1 required%s", "");
     if (!(a->eps >= 0.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: eps >= 0 required%s", "");
     const bool eight = a->state_bits == 8;
-    if (eight && !(a->beta1 * a->beta1 < a->beta2)) return fail(GSR_E_INVALID, "gsr_adamw_step: 8-bit moments need beta1^2 < beta2 (otherwise m / sqrt(v) has no bound)%s", "");
+    if (eight && !opt_spannable(a->beta1, a->beta2)) return fail(GSR_E_INVALID, "gsr_adamw_step: 8-bit moments need beta1^2 < beta2 (otherwise m / sqrt(v) has no bound)%s", "");
     if (a->n_tensors == 0) return 0;
     OptRanges ranges;
     ranges.r.reserve((size_t)a->n_tensors * 6 + 1);
@@ -52,6 +56,8 @@ int adamw_step(const gsr_adamw_args* a)
         const gsr_opt_tensor& t = a->tensors[i];
         if (t.n < 0 || t.n > kOptMaxElements) return fail(GSR_E_INVALID, "gsr_adamw_step: bad tensor size%s", "");
         if (!opt_type_ok(t.param_type) || !opt_type_ok(t.grad_type)) return fail(GSR_E_INVALID, "gsr_adamw_step: unknown type%s", "");
+        if (eight && origins && !opt_spannable(origins[i].beta1, origins[i].beta2))
+            return fail(GSR_E_INVALID, "gsr_adamw_step: the betas of a tensor's codes: 0 <= beta1, beta1^2 < beta2 < 1 required%s", "");
         if (!t.clock || (t.n > 0 && (!t.param || !t.grad || !t.state0 || !t.state1 || (eight && !t.window))))
             return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
         if (((uintptr_t)t.clock & 7) || (((uintptr_t)t.param) & (uintptr_t)(opt_size(t.param_type) - 1)) || (((uintptr_t)t.grad) & (uintptr_t)(opt_size(t.grad_type) - 1)) ||
@@ -73,8 +79,8 @@ int adamw_step(const gsr_adamw_args* a)
     k.beta1 = a->beta1; k.beta2 = a->beta2;
     k.b1 = (float)a->beta1; k.b2 = (float)a->beta2; k.c1 = (float)(1.0 - a->beta1); k.c2 = (float)(1.0 - a->beta2); k.eps = (float)a->eps;
     k.clip = a->clip;
-    const double span = eight ? (1.0 - a->beta1) / sqrt((1.0 - a->beta2) * (1.0 - a->beta1 * a->beta1 / a->beta2)) : 1.0;
-    k.unit = (float)(span / 127.0); k.per_unit = (float)(127.0 / span);
+    const double span = eight ? opt_span(a->beta1, a->beta2) : 1.0;
+    k.per_unit = (float)(127.0 / span);
     for (int i = 0; i < a->n_tensors; ) {
         const int count = std::min(GSR_OPT_MAX, a->n_tensors - i);
         long long bytes = 0;
@@ -89,6 +95,7 @@ int adamw_step(const gsr_adamw_args* a)
             OptTensor& o = k.t[j];
             o.p = t.param; o.g = t.grad; o.s0 = t.state0; o.s1 = t.state1; o.window = t.window; o.clock = t.clock; o.lr_device = t.lr_device;
             o.lr = t.lr; o.decay = t.weight_decay; o.n = t.n; o.first = groups;
+            o.unit = (float)((eight && origins ? opt_span(origins[i].beta1, origins[i].beta2) : span) / 127.0);
             o.key = a->seed * 0x9E3779B1u + (uint32_t)(i + 1) * 0x85EBCA77u;
             const bool aligned = opt_aligned(t.param, opt_size(t.param_type)) && opt_aligned(t.grad, opt_size(t.grad_type)) &&
                                  opt_aligned(t.state0, eight ? 1 : 4) && opt_aligned(t.state1, eight ? 1 : 4);
@@ -117,7 +124,7 @@ int adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1,
     hipStream_t st = (hipStream_t)stream;
     if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return fail(GSR_E_INVALID, "gsr_adamw_moments: NULL pointer%s", "");
     if (!opt_type_ok(type)) return fail(GSR_E_INVALID, "gsr_adamw_moments: unknown type%s", "");
-    if (!(beta1 >= 0.0 && beta2 < 1.0 && beta1 * beta1 < beta2)) return fail(GSR_E_INVALID, "gsr_adamw_moments: 0 <= beta1, beta1^2 < beta2 < 1 required%s", "");
+    if (!opt_spannable(beta1, beta2)) return fail(GSR_E_INVALID, "gsr_adamw_moments: 0 <= beta1, beta1^2 < beta2 < 1 required%s", "");
     OptRanges ranges;
     const void* any = nullptr;
     for (int i = 0; i < n_tensors; i++) {
@@ -134,7 +141,7 @@ int adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1,
     int rc = select_device_of(any);
     if (rc != GSR_OK) return rc;
     MomentArgs k;
-    k.unit = (float)((1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)) / 127.0);
+    k.unit = (float)(opt_span(beta1, beta2) / 127.0);
     k.type = type; k.count = 0;
     uint32_t groups = 0;
     for (int i = 0; i < n_tensors; i++) {

@@ -24,6 +24,7 @@ from . import _lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _OPT = struct.Struct("7Q2dq2i")          # gsr_opt_tensor
+_ORIGIN = struct.Struct("2d")            # gsr_code_origin
 _MOMENT = struct.Struct("5Qq")           # gsr_moment_tensor
 _ROW = struct.Struct("4Qq")              # gsr_row_tensor
 WINDOW = 256                             # elements that share a window byte of the 8-bit root
@@ -121,7 +122,7 @@ def _per_tensor(x, n, name):
     return [x] * n
 
 
-def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed):
+def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, state_betas=None):
     lib = _lib.load()
     n = len(params)
     if not (len(grads) == len(state0) == len(state1) == len(clocks) == n) or (windows is not None and len(windows) != n):
@@ -133,7 +134,11 @@ def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas,
     index = _device(params, name)
     if clip is not None and not (clip.dtype is torch.float32 and clip.numel() == 2 and clip.is_contiguous() and clip.get_device() == index):
         raise ValueError(f"{name}: clip is grad_norm's result (two float32 on the parameters' device)")
-    buf, keep = bytearray(_OPT.size * n), []
+    buf, keep, origins = bytearray(_OPT.size * n), [], None
+    if state_betas is not None:
+        origins = bytearray(_ORIGIN.size * n)
+        for i, (b1, b2) in enumerate(state_betas):
+            _ORIGIN.pack_into(origins, _ORIGIN.size * i, b1, b2)
     for i in range(n):
         p, g, a, b, clock, rate = params[i], grads[i], state0[i], state1[i], clocks[i], lrs[i]
         w = None if windows is None else windows[i]
@@ -158,7 +163,7 @@ def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas,
                        clock.data_ptr(), lr_ptr, rate, decays[i], k, _type(p, name), _type(g, name))
     with _on(index) as stream:
         args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, stream)
-        _lib.check(lib.gsr_adamw_step(C.byref(args)))
+        _lib.check(lib.gsr_adamw_step_coded(C.byref(args), _address(origins)))
     torch.autograd.graph.increment_version([*params, *state0, *state1, *clocks, *(windows or ())])
 
 
@@ -171,20 +176,27 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, clocks, lr, betas=(0.9, 0.9
     """One AdamW step over many tensors in one launch, in place (torch.optim.AdamW; with weight_decay 0 torch.optim.Adam).
     params, grads: float32, bfloat16 or float16; exp_avgs, exp_avg_sqs: float32, zero before the first step; clocks: new_clock() each.
     lr, weight_decay: one number or one per tensor; an lr may be a float64 tensor of one element on the device, which a replayed graph
-    reads anew.  clip: what grad_norm returned, or None.  A gradient that is not contiguous is copied."""
+    reads anew.  clip: what grad_norm returned, or None.  A gradient that is not contiguous is copied.
+    A clock holds the products of its steps' betas; torch's corrections are 1 - beta ** t of the current ones, which differs only where
+    betas change between steps: set clock[0] and clock[1] anew then (AdamW does)."""
     _step(32, "adamw_step", params, grads, exp_avgs, exp_avg_sqs, None, clocks, lr, betas, eps, weight_decay, clip, 0)
 
 
-def adamw_step_8bit(params, grads, rms, ratio, window, clocks, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, clip=None, seed=0):
+def adamw_step_8bit(params, grads, rms, ratio, window, clocks, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, clip=None, seed=0, state_betas=None):
     """adamw_step with a byte for each moment: rms (uint8, sqrt(exp_avg_sq) to a sixteenth of its binade), ratio (int8, exp_avg / sqrt(exp_avg_sq)
     in 127 steps of the largest it can be), window (uint8, one per 256 elements of the flattened tensor: which sixteen binades rms
     covers); all zero before the first step.  Rounding is stochastic, from `seed`, the step and the element's place: the same
-    call on the same state gives the same bits.  Needs beta1^2 < beta2.  moments_8bit reads them."""
-    _step(8, "adamw_step_8bit", params, grads, rms, ratio, window, clocks, lr, betas, eps, weight_decay, clip, seed)
+    call on the same state gives the same bits.  Needs beta1^2 < beta2.  moments_8bit reads them.
+    The largest that the ratio can be depends on the betas.  state_betas: those of the last step that stored the ratios, one pair or one per
+    tensor, where they are not this step's; ratios are read with them and stored with `betas`."""
+    if state_betas is not None:
+        state_betas = _per_tensor(state_betas if isinstance(state_betas[0], (list, tuple)) else [state_betas] * len(params), len(params), "adamw_step_8bit: state_betas")
+    _step(8, "adamw_step_8bit", params, grads, rms, ratio, window, clocks, lr, betas, eps, weight_decay, clip, seed, state_betas)
 
 
 def moments_8bit(rms, ratio, window, betas=(0.9, 0.999), dtype=torch.float32):
-    """The moments that adamw_step_8bit's bytes stand for, as two lists of tensors: exp_avg and sqrt(exp_avg_sq)."""
+    """The moments that adamw_step_8bit's bytes stand for, as two lists of tensors: exp_avg and sqrt(exp_avg_sq).  betas: those of the step that
+    stored them."""
     lib = _lib.load()
     n = len(rms)
     if len(ratio) != n or len(window) != n:
@@ -292,7 +304,12 @@ class AdamW(torch.optim.Optimizer):
     that of their stochastic rounding.  max_norm clips every step by the norm over all groups' gradients, last_norm is then that step's
     (norm, coefficient) on the device.  With 32 bits the state holds "exp_avg" and "exp_avg_sq", shaped like the parameter,
     so code that indexes, concatenates or replaces them goes on working; with 8 bits "rms" and "ratio" are shaped like the parameter and
-    "window" is one byte per 256 elements -- use evict() and append_rows(), which know all of them.  "step" is new_clock()."""
+    "window" is one byte per 256 elements -- use evict() and append_rows(), which know all of them.  "step" is new_clock().
+
+    A group's betas may change between steps, as schedulers do (OneCycleLR): the bias corrections are then torch's, 1 - beta ** t of the current betas, and
+    8-bit ratios are read with the betas that they were stored with.  Those are the group's "state_betas", or the state's own "betas" where it has been
+    stepped with others.  With 8 bits the first step after such a change cannot be captured, and a captured step is not to be replayed after
+    eager ones with other betas."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=32, max_norm=None, seed=0):
         if max_norm is not None and not max_norm >= 0.0:
@@ -321,6 +338,7 @@ class AdamW(torch.optim.Optimizer):
         except ValueError:
             self.param_groups.pop()
             raise
+        g.setdefault("state_betas", tuple(g["betas"]))
 
     def _init_state(self, p, bits):
         if torch.cuda.is_current_stream_capturing():
@@ -341,8 +359,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls, grads = {}, []
+        calls, grads, moved = {}, [], []
         for group in self.param_groups:
+            betas = tuple(group["betas"])
+            home = group.setdefault("state_betas", betas)
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -352,9 +372,16 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state[p] if p in self.state else None
                 if not st:
                     st = self._init_state(p, group["state_bits"])
-                call = calls.setdefault((group["state_bits"], tuple(group["betas"]), group["eps"]), ([], [], [], [], [], [], [], []))
+                    if betas != home:
+                        st["betas"] = betas
+                was = st.get("betas", home)
+                if was != betas:
+                    if group["state_bits"] == 8 and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: the first 8-bit step with other betas cannot be captured (every replay would read the ratios with the old ones): step once before")
+                    moved.append((st, betas, home))
+                call = calls.setdefault((group["state_bits"], betas, group["eps"]), ([], [], [], [], [], [], [], [], []))
                 for x, y in zip(call, (p, p.grad, *((st["exp_avg"], st["exp_avg_sq"], None) if group["state_bits"] == 32 else
-                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"])):
+                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"], was)):
                     x.append(y)
                 grads.append(p.grad)
         if not grads:
@@ -362,8 +389,16 @@ class AdamW(torch.optim.Optimizer):
         clip = None
         if self.max_norm is not None:
             clip = self.last_norm = grad_norm(grads, self.max_norm)
-        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd) in calls.items():
-            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed)
+        for st, betas, home in moved:
+            # torch's corrections: 1 - beta ** t, of this step's betas
+            for k in (0, 1):
+                torch.pow(betas[k], st["step"][2], out=st["step"][k])
+        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, was) in calls.items():
+            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, was if bits == 8 and moved else None)
+        for st, betas, home in moved:
+            st["betas"] = betas
+            if betas == home:
+                del st["betas"]
         return loss
 
     def load_state_dict(self, state_dict):
@@ -382,6 +417,8 @@ class AdamW(torch.optim.Optimizer):
             for k in ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay"):
                 g.pop(k, None)          # (torch.optim.Adam's own options)
             g["state_bits"] = b
+            g["betas"] = tuple(g["betas"])
+            g["state_betas"] = tuple(g.get("state_betas", g["betas"]))
             for i, p in zip(old["params"], g["params"]):
                 if i not in state_dict["state"]:
                     continue

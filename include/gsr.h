@@ -514,9 +514,17 @@ typedef struct gsr_adamw_args {
 /* p <- p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)   with m <- beta1 m + (1 - beta1) g,
  * v <- beta2 v + (1 - beta2) g^2 (torch.optim.AdamW; with weight_decay 0 torch.optim.Adam): computed in 32 bits, half-precision
  * parameters rounded once.  With 8-bit moments the parameter is stepped with the moments before they are rounded; what is stored is
- * described at k_adamw8 (csrc/gsr_mapopt.h).  Memory that a call writes must not overlap other memory of the call: refused. */
+ * described at k_adamw8 (csrc/gsr_mapopt.h).  Memory that a call writes must not overlap other memory of the call: refused.
+ * beta^t is the product over the clock's steps.  Betas may differ from those of earlier steps (a schedule): 32-bit moments go on from
+ * what they are, 8-bit ratios are coded in a unit that depends on the betas, so gsr_adamw_step_coded has to be told which. */
 int gsr_adamw_step(const gsr_adamw_args* args);
-/* The moments that 8-bit codes stand for: exp_avg[i], rms[i] = sqrt(exp_avg_sq)[i] of `type`, dense [n]. */
+/* Of one tensor of an 8-bit step: the betas that its ratio codes were stored with, those of its last step (before its first: any). */
+typedef struct gsr_code_origin { double beta1, beta2; } gsr_code_origin;
+/* gsr_adamw_step where 8-bit codes come from steps of other betas: decoded with those of `origins` (HOST array [n_tensors]; NULL: this
+ * step's), stored with this step's.  32-bit moments have no use for it. */
+int gsr_adamw_step_coded(const gsr_adamw_args* args, const gsr_code_origin* origins);
+/* The moments that 8-bit codes stand for: exp_avg[i], rms[i] = sqrt(exp_avg_sq)[i] of `type`, dense [n]; the betas are those of the
+ * tensors' last step. */
 typedef struct gsr_moment_tensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg_out; void* rms_out; long long n; } gsr_moment_tensor;
 int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream);
 

@@ -91,11 +91,11 @@ def recode(u, window):
     return np.where(place > 0, np.clip(place - 16 * per_block(window, place.size) - 1, 1, 255), 0)
 
 
-def adamw8(p, g, rms, ratio, window, t, lr, betas, eps, decay, coef, seed, place):
+def adamw8(p, g, rms, ratio, window, t, lr, betas, eps, decay, coef, seed, place, state_betas=None):
     """One step on 8-bit moments in 64 bits: p, then the FRACTIONAL places of the new roots and ratios with their random bits added (whose
-    floors are what is stored), and the scales for error bounds."""
+    floors are what is stored), and the scales for error bounds.  state_betas: those that the ratios were stored with, if others."""
     u = decode(rms, window)
-    m = np.asarray(ratio, np.float64).reshape(-1) / 127 * span(*betas) * u
+    m = np.asarray(ratio, np.float64).reshape(-1) / 127 * span(*(state_betas or betas)) * u
     p1, m1, v1, scale = adamw(np.asarray(p).reshape(-1), np.asarray(g).reshape(-1), m, u * u, t, lr, betas, eps, decay, coef)
     du, dr = dither(np.arange(u.size), seed, place, t)
     return p1, m1, np.sqrt(v1), grid_place(np.sqrt(v1)) + du / 2.0 ** 19, dr / 8192.0, scale

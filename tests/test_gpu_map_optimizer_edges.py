@@ -70,3 +70,189 @@ def test_first_8_bit_step_with_a_large_eps(eps):
     MO().adamw_step([p], [g], [torch.zeros_like(p)], [torch.zeros_like(p)], clocks(1, 0, (0.9, 0.999)), lr=1e25, eps=eps)
     MO().adamw_step_8bit([q], [g], [a[0]], [a[1]], [a[2]], clocks(1, 0, (0.9, 0.999)), lr=1e25, eps=eps)
     assert bool(p.isfinite().all()) and torch.equal(p.view(torch.int32), q.view(torch.int32))
+
+
+# ---- betas that change -----------------------------------------------------------------------------------------------------------------
+
+def check8_from(before, after, t, lr, betas, was, eps, place, seed):
+    """One 8-bit step whose ratios were stored with the betas `was`: the parameter by the roundings of a step, the moments within a step of their codes."""
+    p, g, rms, ratio, window = before
+    p1, m1, u1, at, dr, scale = O.adamw8(n64(p), n64(g), rms.cpu().numpy(), ratio.cpu().numpy(), window.cpu().numpy(), t, lr, betas, eps, 0.0, 1.0, seed, place, was)
+    assert (np.abs(n64(after[0]) - p1) <= bound32(p1, m1, None, scale * 1.2, lr, 0.0, torch.float32)).all()
+    codes_, window_ = after[2].cpu().numpy().reshape(-1), after[4].cpu().numpy()
+    u = O.decode(codes_, window_)
+    low = O.decode(np.ones_like(codes_), window_)
+    assert (np.abs(u - u1) <= np.maximum(u1 / 16 * (1 + 64 * E), low)).all() and ((u > 0) == (u1 > 0)).all()
+    unit = O.span(*betas) / 127 * u
+    m = n64(after[3]) * unit          # (a floor of a value with random bits added: under one step off; past 127 steps, 127)
+    size = np.abs(n64(ratio)) / 127 * O.span(*was) * O.decode(rms.cpu().numpy(), window.cpu().numpy()) + np.abs(n64(g))
+    assert (np.abs(m - np.clip(m1, -127 * unit, 127 * unit)) <= unit * (1 + 1e-6) + 20 * E * size).all()
+
+
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.8, 0.95), (0.95, 0.999), (0.0, 0.5), (0.5, 0.3)])
+@pytest.mark.parametrize("was", [None, (0.95, 0.999), (0.85, 0.999), (0.3, 0.9)])
+def test_8_bit_step_of_other_betas(betas, was):
+    n = 5001
+    gen = torch.Generator(device=DEV).manual_seed(53)
+    rms, ratio, window = (x.t for x in random_codes(n, gen, 0, 95, 105))
+    p, g = torch.randn(n, generator=gen, device=DEV), torch.randn(n, generator=gen, device=DEV) * 1e-3 * (torch.rand(n, generator=gen, device=DEV) < 0.7)
+    (avg,), (root,) = MO().moments_8bit([rms], [ratio], [window], betas=was or betas)
+    m = n64(ratio) / 127 * O.span(*(was or betas)) * n64(root)
+    assert (np.abs(n64(avg) - m) <= 3 * E * np.abs(m)).all()
+    ck = clocks(1, 4, betas)
+    first = was or betas
+    for t in (5, 6):
+        before = [x.clone() for x in (p, g, rms, ratio, window)]
+        MO().adamw_step_8bit([p], [g], [rms], [ratio], [window], ck, lr=0.01, betas=betas, eps=1e-12, seed=5, **({} if first == betas else dict(state_betas=first)))
+        check8_from(before, (p, g, rms, ratio, window), t, 0.01, betas, first, 1e-12, 0, 5)
+        first = betas
+    assert abs(float(ck[0][0]) - betas[0] ** 6) < 1e-15 and float(ck[0][2]) == 6
+
+
+def test_state_betas_are_checked():
+    p, a = torch.ones(4, device=DEV), codes(4)
+    ck = clocks(1, 0, (0.9, 0.999))
+    for bad in ((0.99, 0.9), (1.0, 0.999), (-0.1, 0.9), (0.9, 1.0), (float("nan"), 0.9)):
+        with pytest.raises(RuntimeError, match="beta"):
+            MO().adamw_step_8bit([p], [p.clone()], [a[0]], [a[1]], [a[2]], ck, lr=0.1, state_betas=bad)
+    with pytest.raises(ValueError, match="state_betas"):
+        MO().adamw_step_8bit([p], [p.clone()], [a[0]], [a[1]], [a[2]], ck, lr=0.1, state_betas=[(0.9, 0.999)] * 2)
+    assert float(ck[0][2]) == 0.0 and bool((p == 1).all())
+
+
+def cycled(opt, steps):
+    return torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=[0.01 * (i + 1) for i in range(len(opt.param_groups))], total_steps=steps)
+
+
+def test_scheduler_that_cycles_beta1():
+    """torch.optim.lr_scheduler.OneCycleLR sets beta1 anew for every step (0.95 to 0.85 and back): as torch.optim.Adam, whose bias corrections are 1 - beta^t of
+    the betas of the step.  An update's size is under 4 lr: with weights of at most 0.15 the momentum of t gradients is at most 0.15 t of their root mean
+    square (Cauchy-Schwarz), over 1 - 0.95^t that is 3.8 at t = 10.  Its roundings are 40 e of it a step, fed on over 1 / (1 - beta1) <= 20 steps."""
+    gen = torch.Generator(device=DEV).manual_seed(54)
+    ps, opt = small_map(500, gen, 32)
+    qs = [torch.nn.Parameter(p.detach().double().cpu()) for p in ps.values()]
+    ref = torch.optim.Adam([{"params": [q], "lr": 0.01 * (i + 1)} for i, q in enumerate(qs)], lr=0.0, eps=1e-15)
+    sa, sb = cycled(opt, 12), cycled(ref, 12)
+    for t in range(1, 11):
+        for p, q in zip(ps.values(), qs):
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+            q.grad = p.grad.double().cpu()
+        opt.step(); ref.step()
+        b = opt.param_groups[0]["betas"]
+        assert b[0] != 0.9
+        for p in ps.values():
+            c = opt.state[p]["step"].tolist()
+            assert c[0] == pytest.approx(b[0] ** t, rel=1e-14) and c[1] == pytest.approx(b[1] ** t, rel=1e-14) and c[2:] == [t, 0.0]
+        sa.step(); sb.step()
+    for i, (p, q) in enumerate(zip(ps.values(), qs)):
+        assert (np.abs(n64(p) - n64(q)) <= E * (10 * 40 * 4 * 20 * 0.01 * (i + 1) + 30 * np.abs(n64(q)))).all()
+
+
+def step_checked8(opt, gen, missing=()):
+    """One step of an 8-bit optimiser with new gradients, each parameter against the oracle that knows the betas its ratios were stored with."""
+    params = [p for g in opt.param_groups for p in g["params"]]
+    before = []
+    for p in params:
+        st = opt.state.get(p) or {}
+        fresh = codes(p.numel())
+        before.append([p.detach().clone()] + [st[k].clone() if k in st else z for k, z in zip(("rms", "ratio", "window"), fresh)] + [float(st["step"][2]) if st else 0.0])
+        p.grad = None if id(p) in missing else torch.randn(p.shape, generator=gen, device=DEV) * 1e-2
+    opt.step()
+    place = 0
+    for g in opt.param_groups:
+        for p in g["params"]:
+            b, st = before[place], opt.state.get(p)
+            if p.grad is not None:
+                t = int(b[4]) + 1
+                check8_from((b[0], p.grad, b[1], b[2], b[3]), (p, p.grad, st["rms"], st["ratio"], st["window"]), t, g["lr"], g["betas"], p.was if t > 1 else g["betas"], g["eps"], place, opt.seed)
+                assert st["step"].tolist()[0] == pytest.approx(g["betas"][0] ** t, rel=1e-14)
+                p.was = g["betas"]
+            place += 1
+
+
+def test_8_bit_optimizer_under_cycled_betas():
+    """... through steps that leave a parameter out (its ratios keep the betas they were stored with), an eviction, copies, pickles and a state dict"""
+    gen = torch.Generator(device=DEV).manual_seed(55)
+    ps, opt = small_map(300, gen, 8, seed=9)
+    sched = cycled(opt, 40)
+    left_out = ps["opacity"]
+    for t in range(1, 6):
+        step_checked8(opt, gen, (id(left_out),) if t in (2, 3) else ())
+        sched.step()
+
+    def follow(other, params):
+        for p, q in zip([p for g in opt.param_groups for p in g["params"]], params):
+            q.was = p.was
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        follow(other, [q for g in other.param_groups for q in g["params"]])
+        step_checked8(other, gen)
+    saved = opt.state_dict()
+    saved = dict(saved, state={i: {k: v.cpu().clone() if torch.is_tensor(v) else v for k, v in s.items()} for i, s in saved["state"].items()})
+    qs, other = small_map(300, gen, 8, seed=9)
+    with torch.no_grad():
+        for p, q in zip(ps.values(), qs.values()):
+            q.copy_(p)
+    other.load_state_dict(saved)
+    follow(other, qs.values())
+    for g in other.param_groups:
+        g["betas"] = (0.7, 0.99)
+    step_checked8(other, gen)
+    was = [p.was for g in opt.param_groups for p in g["params"]]
+    opt.evict(torch.rand(300, generator=gen, device=DEV), 200)
+    for p, w in zip((p for g in opt.param_groups for p in g["params"]), was):
+        p.was = w
+    sched.step()
+    step_checked8(opt, gen)
+
+
+def test_changed_betas_are_not_captured_with_8_bits():
+    """a replay would decode with the betas from before again and again"""
+    p = torch.nn.Parameter(torch.ones(500, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = MO().AdamW([p], lr=0.1, state_bits=8)
+    opt.step()
+    opt.param_groups[0]["betas"] = (0.8, 0.99)
+    before = [x.clone() for x in (p.detach(), *(opt.state[p][k] for k in ("rms", "ratio", "window", "step")))]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    for x, y in zip(before, (p.detach(), *(opt.state[p][k] for k in ("rms", "ratio", "window", "step")))):
+        assert torch.equal(x, y)
+    opt.step()          # eagerly, and from then on captured
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    other = copy.deepcopy(opt)
+    q = other.param_groups[0]["params"][0]
+    for _ in range(3):
+        graph.replay()
+        q.grad = torch.ones_like(q)
+        other.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["ratio"], other.state[q]["ratio"])
+
+
+def test_changed_betas_captured_with_32_bits():
+    """every replay forms its corrections from the count and the betas of the capture, as an eager step that follows one with the same betas: the
+    powers agree to a few 2^-53, the parameters to the roundings of four steps (40 e of an update of the rate's size each)"""
+    p = torch.nn.Parameter(torch.linspace(-1, 1, 500, device=DEV))
+    p.grad = torch.linspace(-2, 1, 500, device=DEV)
+    opt = MO().AdamW([p], lr=0.1)
+    opt.step()
+    opt.param_groups[0]["betas"] = (0.8, 0.99)
+    torch.cuda.synchronize()
+    other = copy.deepcopy(opt)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    q = other.param_groups[0]["params"][0]
+    q.grad = p.grad.clone()
+    for t in range(2, 6):
+        graph.replay()
+        other.step()
+        torch.cuda.synchronize()
+        a, b = opt.state[p]["step"].tolist(), other.state[q]["step"].tolist()
+        assert a[2:] == b[2:] == [t, 0.0] and a[:2] == pytest.approx([0.8 ** t, 0.99 ** t], rel=1e-14) and b[:2] == pytest.approx(a[:2], rel=1e-14)
+        assert float((p - q).abs().max()) <= E * (4 * 40 * 0.2 + 4 * 2)
