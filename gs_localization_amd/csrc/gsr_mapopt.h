@@ -167,7 +167,7 @@ struct OptTensor {
     double lr, decay;
     long long n;
     uint32_t first;             // its first workgroup in the launch
-    uint32_t key;               // 8 bits: seed and place in the list
+    uint32_t key;               // 8 bits: seed and place
     int types;                  // parameter | gradient << 4 | GSR_T_ALIGNED
     float unit;                 // 8 bits: the step of the ratios that it comes with (of the betas they were stored with)
 };

@@ -96,7 +96,7 @@ int adamw_step(const gsr_adamw_args* a, const gsr_code_origin* origins)
             o.p = t.param; o.g = t.grad; o.s0 = t.state0; o.s1 = t.state1; o.window = t.window; o.clock = t.clock; o.lr_device = t.lr_device;
             o.lr = t.lr; o.decay = t.weight_decay; o.n = t.n; o.first = groups;
             o.unit = (float)((eight && origins ? opt_span(origins[i].beta1, origins[i].beta2) : span) / 127.0);
-            o.key = a->seed * 0x9E3779B1u + (uint32_t)(i + 1) * 0x85EBCA77u;
+            o.key = a->seed * 0x9E3779B1u + ((eight && origins ? origins[i].place : (uint32_t)i) + 1u) * 0x85EBCA77u;
             const bool aligned = opt_aligned(t.param, opt_size(t.param_type)) && opt_aligned(t.grad, opt_size(t.grad_type)) &&
                                  opt_aligned(t.state0, eight ? 1 : 4) && opt_aligned(t.state1, eight ? 1 : 4);
             o.types = t.param_type | t.grad_type << 4 | (aligned ? GSR_T_ALIGNED : 0);

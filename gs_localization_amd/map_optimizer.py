@@ -24,7 +24,7 @@ from . import _lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _OPT = struct.Struct("7Q2dq2i")          # gsr_opt_tensor
-_ORIGIN = struct.Struct("2d")            # gsr_code_origin
+_ORIGIN = struct.Struct("2dI4x")         # gsr_code_origin
 _MOMENT = struct.Struct("5Qq")           # gsr_moment_tensor
 _ROW = struct.Struct("4Qq")              # gsr_row_tensor
 WINDOW = 256                             # elements that share a window byte of the 8-bit root
@@ -122,7 +122,7 @@ def _per_tensor(x, n, name):
     return [x] * n
 
 
-def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, state_betas=None):
+def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, origin=None):
     lib = _lib.load()
     n = len(params)
     if not (len(grads) == len(state0) == len(state1) == len(clocks) == n) or (windows is not None and len(windows) != n):
@@ -135,10 +135,10 @@ def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas,
     if clip is not None and not (clip.dtype is torch.float32 and clip.numel() == 2 and clip.is_contiguous() and clip.get_device() == index):
         raise ValueError(f"{name}: clip is grad_norm's result (two float32 on the parameters' device)")
     buf, keep, origins = bytearray(_OPT.size * n), [], None
-    if state_betas is not None:
+    if origin is not None:          # (8 bits) a tensor's: the betas it was stored with, its place
         origins = bytearray(_ORIGIN.size * n)
-        for i, (b1, b2) in enumerate(state_betas):
-            _ORIGIN.pack_into(origins, _ORIGIN.size * i, b1, b2)
+        for i, ((b1, b2), place) in enumerate(origin):
+            _ORIGIN.pack_into(origins, _ORIGIN.size * i, b1, b2, place)
     for i in range(n):
         p, g, a, b, clock, rate = params[i], grads[i], state0[i], state1[i], clocks[i], lrs[i]
         w = None if windows is None else windows[i]
@@ -185,13 +185,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, clocks, lr, betas=(0.9, 0.9
 def adamw_step_8bit(params, grads, rms, ratio, window, clocks, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, clip=None, seed=0, state_betas=None):
     """adamw_step with a byte for each moment: rms (uint8, sqrt(exp_avg_sq) to a sixteenth of its binade), ratio (int8, exp_avg / sqrt(exp_avg_sq)
     in 127 steps of the largest it can be), window (uint8, one per 256 elements of the flattened tensor: which sixteen binades rms
-    covers); all zero before the first step.  Rounding is stochastic, from `seed`, the step and the element's place: the same
+    covers); all zero before the first step.  Rounding is stochastic, from `seed`, the step, the tensor's place in the list and the element's: the same
     call on the same state gives the same bits.  Needs beta1^2 < beta2.  moments_8bit reads them.
     The largest that the ratio can be depends on the betas.  state_betas: those of the last step that stored the ratios, one pair or one per
     tensor, where they are not this step's; ratios are read with them and stored with `betas`."""
     if state_betas is not None:
         state_betas = _per_tensor(state_betas if isinstance(state_betas[0], (list, tuple)) else [state_betas] * len(params), len(params), "adamw_step_8bit: state_betas")
-    _step(8, "adamw_step_8bit", params, grads, rms, ratio, window, clocks, lr, betas, eps, weight_decay, clip, seed, state_betas)
+    _step(8, "adamw_step_8bit", params, grads, rms, ratio, window, clocks, lr, betas, eps, weight_decay, clip, seed,
+          None if state_betas is None else zip(state_betas, range(len(params))))
 
 
 def moments_8bit(rms, ratio, window, betas=(0.9, 0.999), dtype=torch.float32):
@@ -301,10 +302,11 @@ class AdamW(torch.optim.Optimizer):
     training_setup (gaussian_splatting/scene/gaussian_model.py:149-167) has `torch.optim.Adam(groups, lr=0.0, eps=1e-15)`.
 
     weight_decay is decoupled (0, Adam, by default).  state_bits=8 (per group) keeps the moments in two bytes per element; seed is
-    that of their stochastic rounding.  max_norm clips every step by the norm over all groups' gradients, last_norm is then that step's
-    (norm, coefficient) on the device.  With 32 bits the state holds "exp_avg" and "exp_avg_sq", shaped like the parameter,
-    so code that indexes, concatenates or replaces them goes on working; with 8 bits "rms" and "ratio" are shaped like the parameter and
-    "window" is one byte per 256 elements -- use evict() and append_rows(), which know all of them.  "step" is new_clock().
+    that of their stochastic rounding (with the step and a parameter's place among all of the optimiser's).  max_norm clips every step by the
+    norm over all groups' gradients, last_norm is then that step's (norm, coefficient) on the device.  With 32 bits the state holds
+    "exp_avg" and "exp_avg_sq", shaped like the parameter, so code that indexes, concatenates or replaces them goes on working; with 8 bits
+    "rms" and "ratio" are shaped like the parameter and "window" is one byte per 256 elements -- use evict() and append_rows(), which know
+    all of them.  "step" is new_clock().
 
     A group's betas may change between steps, as schedulers do (OneCycleLR): the bias corrections are then torch's, 1 - beta ** t of the current betas, and
     8-bit ratios are read with the betas that they were stored with.  Those are the group's "state_betas", or the state's own "betas" where it has been
@@ -359,11 +361,12 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls, grads, moved = {}, [], []
+        calls, grads, moved, place = {}, [], [], -1
         for group in self.param_groups:
             betas = tuple(group["betas"])
             home = group.setdefault("state_betas", betas)
             for p in group["params"]:
+                place += 1          # (of a parameter, whichever others are stepped and in how many calls: its random bits are its own)
                 if p.grad is None:
                     continue
                 if p.grad.layout is not torch.strided:
@@ -381,7 +384,7 @@ class AdamW(torch.optim.Optimizer):
                     moved.append((st, betas, home))
                 call = calls.setdefault((group["state_bits"], betas, group["eps"]), ([], [], [], [], [], [], [], [], []))
                 for x, y in zip(call, (p, p.grad, *((st["exp_avg"], st["exp_avg_sq"], None) if group["state_bits"] == 32 else
-                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"], was)):
+                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"], (was, place))):
                     x.append(y)
                 grads.append(p.grad)
         if not grads:
@@ -393,8 +396,8 @@ class AdamW(torch.optim.Optimizer):
             # torch's corrections: 1 - beta ** t, of this step's betas
             for k in (0, 1):
                 torch.pow(betas[k], st["step"][2], out=st["step"][k])
-        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, was) in calls.items():
-            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, was if bits == 8 and moved else None)
+        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, origin) in calls.items():
+            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, origin if bits == 8 else None)
         for st, betas, home in moved:
             st["betas"] = betas
             if betas == home:

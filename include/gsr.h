@@ -518,10 +518,11 @@ typedef struct gsr_adamw_args {
  * beta^t is the product over the clock's steps.  Betas may differ from those of earlier steps (a schedule): 32-bit moments go on from
  * what they are, 8-bit ratios are coded in a unit that depends on the betas, so gsr_adamw_step_coded has to be told which. */
 int gsr_adamw_step(const gsr_adamw_args* args);
-/* Of one tensor of an 8-bit step: the betas that its ratio codes were stored with, those of its last step (before its first: any). */
-typedef struct gsr_code_origin { double beta1, beta2; } gsr_code_origin;
+/* Of one tensor of an 8-bit step: the betas that its ratio codes were stored with, those of its last step (before its first: any), and its
+ * place, which with the seed and the step says by which random bits it rounds. */
+typedef struct gsr_code_origin { double beta1, beta2; unsigned place; } gsr_code_origin;
 /* gsr_adamw_step where 8-bit codes come from steps of other betas: decoded with those of `origins` (HOST array [n_tensors]; NULL: this
- * step's), stored with this step's.  32-bit moments have no use for it. */
+ * step's betas, places in the list), stored with this step's.  32-bit moments have no use for it. */
 int gsr_adamw_step_coded(const gsr_adamw_args* args, const gsr_code_origin* origins);
 /* The moments that 8-bit codes stand for: exp_avg[i], rms[i] = sqrt(exp_avg_sq)[i] of `type`, dense [n]; the betas are those of the
  * tensors' last step. */

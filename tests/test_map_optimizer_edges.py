@@ -14,7 +14,7 @@ def coded(origin, **kw):
     buf, origins = bytearray(MO._OPT.size), bytearray(MO._ORIGIN.size)
     MO._OPT.pack_into(buf, 0, *dict(dict(param=0x1000, grad=0x20000, state0=0x30000, state1=0x40000, window=0x50000, clock=0x60000, lr_device=0, lr=0.1, decay=0.0,
                                          n=64, pt=0, gt=0), **kw).values())
-    MO._ORIGIN.pack_into(origins, 0, *origin)
+    MO._ORIGIN.pack_into(origins, 0, *origin, 0)
     args = _lib.AdamwArgs(1, 8, MO._address(buf), 0.9, 0.999, 1e-8, None, 0, None)
     return lib.gsr_adamw_step_coded(C.byref(args), MO._address(origins)), lib.gsr_last_error().decode()
 
