@@ -143,6 +143,7 @@ SIGNATURES.update({
     "gsr_grad_norm": (_i, [_i, C.POINTER(_vp), C.POINTER(C.c_longlong), C.POINTER(_i), _f, _vp, RESIZE_FN, _vp, _vp]),
     "gsr_adamw_step": (_i, [C.POINTER(AdamwArgs)]),
     "gsr_adamw_step_coded": (_i, [C.POINTER(AdamwArgs), _vp]),
+    "gsr_adamw_check": (_i, [C.POINTER(AdamwArgs), _vp]),
     "gsr_adamw_moments": (_i, [_i, _vp, C.c_double, C.c_double, _i, _vp]),
     "gsr_evict_bytes": (C.c_size_t, [_i]),
     "gsr_evict_rows": (_i, [C.POINTER(EvictArgs)]),

@@ -2084,6 +2084,12 @@ int gsr_adamw_step_coded(const gsr_adamw_args* args, const gsr_code_origin* orig
     return no_throw([&] { return adamw_step(args, origins); });
 }
 
+int gsr_adamw_check(const gsr_adamw_args* args, const gsr_code_origin* origins)
+{
+    if (!args) return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
+    return no_throw([&] { return adamw_check(args, origins); });
+}
+
 int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream)
 {
     return no_throw([&] { return adamw_moments(n_tensors, tensors, beta1, beta2, type, stream); });

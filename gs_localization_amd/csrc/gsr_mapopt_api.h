@@ -38,18 +38,14 @@ struct OptRanges {
 bool opt_spannable(double beta1, double beta2) { return beta1 >= 0.0 && beta1 * beta1 < beta2 && beta2 < 1.0; }
 double opt_span(double beta1, double beta2) { return (1.0 - beta1) / sqrt((1.0 - beta2) * (1.0 - beta1 * beta1 / beta2)); }
 
-int adamw_step(const gsr_adamw_args* a, const gsr_code_origin* origins)
+int adamw_check(const gsr_adamw_args* a, const gsr_code_origin* origins)
 {
-    using namespace gsr;
-    const int debug = 0;
-    hipStream_t st = (hipStream_t)a->stream;
     if (a->n_tensors < 0 || (a->n_tensors > 0 && !a->tensors)) return fail(GSR_E_INVALID, "gsr_adamw_step: NULL pointer%s", "");
     if (a->state_bits != 32 && a->state_bits != 8) return fail(GSR_E_INVALID, "gsr_adamw_step: moments have 32 or 8 bits%s", "");
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: 0 <= beta < 1 required%s", "");
     if (!(a->eps >= 0.0)) return fail(GSR_E_INVALID, "gsr_adamw_step: eps >= 0 required%s", "");
     const bool eight = a->state_bits == 8;
     if (eight && !opt_spannable(a->beta1, a->beta2)) return fail(GSR_E_INVALID, "gsr_adamw_step: 8-bit moments need beta1^2 < beta2 (otherwise m / sqrt(v) has no bound)%s", "");
-    if (a->n_tensors == 0) return 0;
     OptRanges ranges;
     ranges.r.reserve((size_t)a->n_tensors * 6 + 1);
     for (int i = 0; i < a->n_tensors; i++) {
@@ -73,7 +69,18 @@ int adamw_step(const gsr_adamw_args* a, const gsr_code_origin* origins)
     }
     ranges.add(a->clip, 2 * sizeof(float), false);
     if (ranges.clash()) return fail(GSR_E_INVALID, "gsr_adamw_step: memory that the step writes overlaps other memory of the call (a tensor given twice?)%s", "");
-    int rc = select_device_of(a->tensors[0].clock);
+    return GSR_OK;
+}
+
+int adamw_step(const gsr_adamw_args* a, const gsr_code_origin* origins)
+{
+    using namespace gsr;
+    const int debug = 0;
+    hipStream_t st = (hipStream_t)a->stream;
+    const bool eight = a->state_bits == 8;
+    int rc = adamw_check(a, origins);
+    if (rc != GSR_OK || a->n_tensors == 0) return rc;
+    rc = select_device_of(a->tensors[0].clock);
     if (rc != GSR_OK) return rc;
     OptArgs k;
     k.beta1 = a->beta1; k.beta2 = a->beta2;

@@ -122,13 +122,26 @@ def _per_tensor(x, n, name):
     return [x] * n
 
 
-def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, origin=None):
-    lib = _lib.load()
+class _Call:
+    """A checked and packed call of gsr_adamw_step_coded, and what has to stay alive until it is made."""
+    __slots__ = ("args", "origins", "index", "written", "held")
+
+    def check(self):
+        _lib.check(_lib.load().gsr_adamw_check(C.byref(self.args), _address(self.origins)))
+
+    def launch(self):
+        with _on(self.index) as stream:
+            self.args.stream = stream
+            _lib.check(_lib.load().gsr_adamw_step_coded(C.byref(self.args), _address(self.origins)))
+        torch.autograd.graph.increment_version(self.written)
+
+
+def _pack(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, origin=None):
     n = len(params)
     if not (len(grads) == len(state0) == len(state1) == len(clocks) == n) or (windows is not None and len(windows) != n):
         raise ValueError(f"{name}: lists of different lengths")
     if n == 0:
-        return
+        return None
     lrs, decays = _per_tensor(lr, n, name + ": lr"), _per_tensor(weight_decay, n, name + ": weight_decay")
     d0, d1 = (torch.float32, torch.float32) if bits == 32 else (torch.uint8, torch.int8)
     index = _device(params, name)
@@ -161,10 +174,17 @@ def _step(bits, name, params, grads, state0, state1, windows, clocks, lr, betas,
             lr_ptr, rate = rate.data_ptr(), 0.0
         _OPT.pack_into(buf, _OPT.size * i, p.data_ptr(), g.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if w is None else w.data_ptr(),
                        clock.data_ptr(), lr_ptr, rate, decays[i], k, _type(p, name), _type(g, name))
-    with _on(index) as stream:
-        args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, stream)
-        _lib.check(lib.gsr_adamw_step_coded(C.byref(args), _address(origins)))
-    torch.autograd.graph.increment_version([*params, *state0, *state1, *clocks, *(windows or ())])
+    call = _Call()
+    call.args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, None)
+    call.origins, call.index, call.held = origins, index, (buf, keep, clip)
+    call.written = [*params, *state0, *state1, *clocks, *(windows or ())]
+    return call
+
+
+def _step(*args):
+    call = _pack(*args)
+    if call is not None:
+        call.launch()
 
 
 def new_clock(device):
@@ -389,19 +409,25 @@ class AdamW(torch.optim.Optimizer):
                 grads.append(p.grad)
         if not grads:
             return loss
-        clip = None
-        if self.max_norm is not None:
-            clip = self.last_norm = grad_norm(grads, self.max_norm)
+        clip = None if self.max_norm is None else grad_norm(grads, self.max_norm)
+        # (made whole or not at all: everything is checked before anything is launched)
+        packed = [_pack(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, origin if bits == 8 else None)
+                  for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, origin) in calls.items()]
+        if len(packed) > 1 or moved:
+            for call in packed:
+                call.check()
         for st, betas, home in moved:
             # torch's corrections: 1 - beta ** t, of this step's betas
             for k in (0, 1):
                 torch.pow(betas[k], st["step"][2], out=st["step"][k])
-        for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, origin) in calls.items():
-            _step(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, origin if bits == 8 else None)
+        for call in packed:
+            call.launch()
         for st, betas, home in moved:
             st["betas"] = betas
             if betas == home:
                 del st["betas"]
+        if clip is not None:
+            self.last_norm = clip
         return loss
 
     def load_state_dict(self, state_dict):

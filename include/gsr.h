@@ -524,6 +524,8 @@ typedef struct gsr_code_origin { double beta1, beta2; unsigned place; } gsr_code
 /* gsr_adamw_step where 8-bit codes come from steps of other betas: decoded with those of `origins` (HOST array [n_tensors]; NULL: this
  * step's betas, places in the list), stored with this step's.  32-bit moments have no use for it. */
 int gsr_adamw_step_coded(const gsr_adamw_args* args, const gsr_code_origin* origins);
+/* What gsr_adamw_step_coded would refuse, without a launch: for an optimiser whose step takes several calls and is made whole or not at all. */
+int gsr_adamw_check(const gsr_adamw_args* args, const gsr_code_origin* origins);
 /* The moments that 8-bit codes stand for: exp_avg[i], rms[i] = sqrt(exp_avg_sq)[i] of `type`, dense [n]; the betas are those of the
  * tensors' last step. */
 typedef struct gsr_moment_tensor { const uint8_t* rms; const int8_t* ratio; const uint8_t* window; void* exp_avg_out; void* rms_out; long long n; } gsr_moment_tensor;

@@ -290,3 +290,37 @@ def test_changed_betas_captured_with_32_bits():
         a, b = opt.state[p]["step"].tolist(), other.state[q]["step"].tolist()
         assert a[2:] == b[2:] == [t, 0.0] and a[:2] == pytest.approx([0.8 ** t, 0.99 ** t], rel=1e-14) and b[:2] == pytest.approx(a[:2], rel=1e-14)
         assert float((p - q).detach().abs().max()) <= E * (4 * 40 * 0.2 + 4 * 2)
+
+
+# ---- refused as a whole ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("what", ["type", "betas", "overlap", "size"])
+def test_a_refused_step_has_stepped_nothing(bits, what):
+    gen = torch.Generator(device=DEV).manual_seed(56)
+    ps = [torch.nn.Parameter(torch.randn(500, generator=gen, device=DEV)) for _ in range(3)]
+    opt = MO().AdamW([{"params": ps[:1]}, {"params": ps[1:2], "eps": 1e-3}, {"params": ps[2:], "eps": 1e-4}], lr=0.1, state_bits=bits, max_norm=1.0)
+    for p in ps:
+        p.grad = torch.randn(500, generator=gen, device=DEV)
+    opt.step()
+    st, k = opt.state[ps[1]], "exp_avg" if bits == 32 else "ratio"
+    good, betas = dict(st), opt.param_groups[1]["betas"]
+    if what == "type":
+        st[k] = st[k].bfloat16()
+    elif what == "betas":
+        opt.param_groups[1]["betas"] = (1.0, 0.999)
+    elif what == "overlap":
+        st["step"] = ps[1].detach()[2:10].view(torch.float64)          # (its own, and yet in the parameter)
+    else:
+        st[k] = st[k][:400]
+    watched = [x for p in ps for x in (p.detach(), *(y for y in opt.state[p].values() if torch.is_tensor(y)))]
+    before = [x.clone() for x in watched]
+    with pytest.raises((RuntimeError, TypeError, ValueError)):
+        opt.step()
+    torch.cuda.synchronize()
+    for x, y in zip(watched, before):
+        assert torch.equal(x, y)
+    opt.param_groups[1]["betas"] = betas
+    opt.state[ps[1]] = good
+    opt.step()
+    assert [float(opt.state[p]["step"][2]) for p in ps] == [2.0] * 3

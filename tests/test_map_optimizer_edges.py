@@ -16,7 +16,10 @@ def coded(origin, **kw):
                                          n=64, pt=0, gt=0), **kw).values())
     MO._ORIGIN.pack_into(origins, 0, *origin, 0)
     args = _lib.AdamwArgs(1, 8, MO._address(buf), 0.9, 0.999, 1e-8, None, 0, None)
-    return lib.gsr_adamw_step_coded(C.byref(args), MO._address(origins)), lib.gsr_last_error().decode()
+    checked, said = lib.gsr_adamw_check(C.byref(args), MO._address(origins)), lib.gsr_last_error().decode()
+    rc = lib.gsr_adamw_step_coded(C.byref(args), MO._address(origins))
+    assert checked == (0 if rc == -4 else rc) and (rc == -4 or said == lib.gsr_last_error().decode())
+    return rc, lib.gsr_last_error().decode()
 
 
 def test_betas_of_the_codes_are_checked():
