@@ -431,12 +431,15 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Takes its own state_dict() and torch.optim.Adam's / AdamW's (32-bit groups): states keep their types whatever the parameter's."""
+        """Takes its own state_dict() and torch.optim.Adam's / AdamW's (32-bit groups): states keep their types whatever the parameter's.
+        weight_decay is decoupled here: a group of torch's that has one must say that its is ("decoupled_weight_decay"; torch's AdamW does)."""
         own, given = self.param_groups, state_dict["param_groups"]
         bits = [g.get("state_bits", own[k]["state_bits"]) if k < len(own) else 32 for k, g in enumerate(given)]
         for b, g in zip(bits, given):
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("load_state_dict: amsgrad and maximize are not supported")
+            if g.get("weight_decay") and not g.get("decoupled_weight_decay", "state_bits" in g):
+                raise ValueError("load_state_dict: a group's weight_decay is not decoupled, or its state_dict does not say (if it is, set the group's decoupled_weight_decay to True)")
             wanted = {"exp_avg", "exp_avg_sq", "step"} if b == 32 else {"rms", "ratio", "window", "step"}
             for i in g["params"]:
                 if i in state_dict["state"] and not wanted <= set(state_dict["state"][i]):

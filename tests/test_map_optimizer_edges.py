@@ -47,3 +47,35 @@ def test_state_dict_without_the_betas_of_its_codes():
     opt = MO.AdamW([torch.nn.Parameter(torch.zeros(4))], state_bits=8)
     opt.load_state_dict(saved)
     assert opt.param_groups[0]["state_betas"] == (0.8, 0.95)
+
+
+def trained(cls, old=False, **kw):
+    """The state_dict of torch's optimiser after a step; old: as releases before "decoupled_weight_decay" wrote it."""
+    p = torch.nn.Parameter(torch.ones(4))
+    p.grad = torch.ones(4)
+    ref = cls([p], lr=0.1, **kw)
+    ref.step()
+    saved = ref.state_dict()
+    for g in saved["param_groups"]:
+        if old:
+            del g["decoupled_weight_decay"]
+    return saved
+
+
+def test_decay_that_is_added_to_the_gradient_is_refused():
+    """torch.optim.Adam's weight_decay is, AdamW's is not: the same number means another step"""
+    opt = MO.AdamW([torch.nn.Parameter(torch.zeros(4))], lr=0.3)
+    for saved in (trained(torch.optim.Adam, weight_decay=0.1), trained(torch.optim.Adam, old=True, weight_decay=0.1), trained(torch.optim.AdamW, old=True)):
+        with pytest.raises(ValueError, match="decoupled"):
+            opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] == 0.3 and opt.param_groups[0]["weight_decay"] == 0.0 and not opt.state
+    for saved, decay in ((trained(torch.optim.Adam), 0.0), (trained(torch.optim.Adam, old=True), 0.0), (trained(torch.optim.AdamW, weight_decay=0.1), 0.1),
+                         (trained(torch.optim.Adam, decoupled_weight_decay=True, weight_decay=0.2), 0.2), (opt.state_dict(), 0.0),
+                         (MO.AdamW([torch.nn.Parameter(torch.zeros(4))], weight_decay=0.4).state_dict(), 0.4)):
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["weight_decay"] == decay and "decoupled_weight_decay" not in opt.param_groups[0]
+    # which it is can be said where the file does not
+    saved = trained(torch.optim.AdamW, old=True, weight_decay=0.1)
+    saved["param_groups"][0]["decoupled_weight_decay"] = True
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["weight_decay"] == 0.1
