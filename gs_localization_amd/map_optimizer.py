@@ -88,6 +88,12 @@ def _workspace(nbytes, index):
     return t, _lib.FixedBuffer(t.data_ptr(), nbytes, 0)
 
 
+def _dense(t):
+    """A dense tensor of t's values: strides, and what torch has only marked (a conjugate; the sign of its imaginary part, which is contiguous if it
+    is one element), are copied."""
+    return t.resolve_conj().resolve_neg().contiguous()
+
+
 def _address(buf):
     return C.addressof(C.c_char.from_buffer(buf)) if buf else None
 
@@ -97,7 +103,7 @@ def grad_norm(grads, max_norm=math.inf):
     all of them (64-bit sums in a fixed order) and min(1, max_norm / (norm + 1e-6)), what torch.nn.utils.clip_grad_norm_ would multiply them
     by -- handed to adamw_step as `clip` no gradient is written.  A NaN or infinite gradient gives a norm that says so."""
     lib = _lib.load()
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    grads = [g if g.is_contiguous() and not g.is_neg() else _dense(g) for g in grads]
     if not grads:
         raise ValueError("grad_norm: no gradients")
     if not max_norm >= 0.0:
@@ -122,21 +128,8 @@ def _per_tensor(x, n, name):
     return [x] * n
 
 
-class _Call:
-    """A checked and packed call of gsr_adamw_step_coded, and what has to stay alive until it is made."""
-    __slots__ = ("args", "origins", "index", "written", "held")
-
-    def check(self):
-        _lib.check(_lib.load().gsr_adamw_check(C.byref(self.args), _address(self.origins)))
-
-    def launch(self):
-        with _on(self.index) as stream:
-            self.args.stream = stream
-            _lib.check(_lib.load().gsr_adamw_step_coded(C.byref(self.args), _address(self.origins)))
-        torch.autograd.graph.increment_version(self.written)
-
-
 def _pack(bits, name, params, grads, state0, state1, windows, clocks, lr, betas, eps, weight_decay, clip, seed, origin=None):
+    """A call of gsr_adamw_step_coded for _launch, its tensors checked; None without tensors."""
     n = len(params)
     if not (len(grads) == len(state0) == len(state1) == len(clocks) == n) or (windows is not None and len(windows) != n):
         raise ValueError(f"{name}: lists of different lengths")
@@ -164,27 +157,38 @@ def _pack(bits, name, params, grads, state0, state1, windows, clocks, lr, betas,
             raise ValueError(f"{name}: tensor {i}: sizes do not match the parameter's {tuple(p.shape)}")
         if not (p.is_contiguous() and a.is_contiguous() and b.is_contiguous() and clock.is_contiguous() and (w is None or w.is_contiguous())):
             raise ValueError(f"{name}: tensor {i}: what the step writes must be contiguous")
-        if not g.is_contiguous():
-            g = g.contiguous()
+        if k == 1 and p.is_neg():
+            raise ValueError(f"{name}: tensor {i}: the parameter is marked as a negative: resolve_neg() first")
+        if not g.is_contiguous() or (k == 1 and g.is_neg()):
+            g = _dense(g)
             keep.append(g)
+        pt, gt = _TYPES.get(p.dtype), _TYPES.get(g.dtype)
+        if pt is None or gt is None:
+            _type(p, name), _type(g, name)
         lr_ptr = 0
         if not isinstance(rate, float) and torch.is_tensor(rate):
             if not (rate.dtype is torch.float64 and rate.numel() == 1 and rate.get_device() == index):
                 raise ValueError(f"{name}: lr as a tensor is one float64 on the parameters' device")
             lr_ptr, rate = rate.data_ptr(), 0.0
         _OPT.pack_into(buf, _OPT.size * i, p.data_ptr(), g.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if w is None else w.data_ptr(),
-                       clock.data_ptr(), lr_ptr, rate, decays[i], k, _type(p, name), _type(g, name))
-    call = _Call()
-    call.args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, None)
-    call.origins, call.index, call.held = origins, index, (buf, keep, clip)
-    call.written = [*params, *state0, *state1, *clocks, *(windows or ())]
-    return call
+                       clock.data_ptr(), lr_ptr, rate, decays[i], k, pt, gt)
+    args = _lib.AdamwArgs(n, bits, _address(buf), betas[0], betas[1], eps, None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF, None)
+    # (the last: what has to stay alive until the launch)
+    return args, origins, index, [*params, *state0, *state1, *clocks, *(windows or ())], (buf, keep, clip)
+
+
+def _launch(call):
+    args, origins, index, written, _ = call
+    with _on(index) as stream:
+        args.stream = stream
+        _lib.check(_lib.load().gsr_adamw_step_coded(C.byref(args), _address(origins)))
+    torch.autograd.graph.increment_version(written)
 
 
 def _step(*args):
     call = _pack(*args)
     if call is not None:
-        call.launch()
+        _launch(call)
 
 
 def new_clock(device):
@@ -261,27 +265,27 @@ def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=())
     if P > 0x7FFFFFFF:
         raise ValueError("evict_rows: at most 2^31 - 1 rows")
     if weights is not None:
-        weights = (weights if weights.dim() == 2 else weights.unsqueeze(0)).contiguous()
+        weights = _dense(weights if weights.dim() == 2 else weights.unsqueeze(0))
         if weights.dtype is not torch.float32 or weights.dim() != 2 or weights.shape[1] != P:
             raise ValueError("evict_rows: weights is float32 [views, P] or [P]")
-    scores = scores.contiguous()
+    scores = _dense(scores)
     index = _device([scores, *(() if weights is None else (weights,)), *tensors, *[x for pair in rms for x in pair]], "evict_rows")
     n, size = len(tensors) + len(rms), _ROW.size
     buf, rows, pairs, held = bytearray(size * n), [], [], []
     with _on(index) as stream:
         out = scores.new_empty(keep)
         kept = torch.empty(keep, dtype=torch.int64, device=scores.device)
-        at = 0
+        at, pack = 0, _ROW.pack_into
         for t in tensors:
             shape = t.shape
             if not shape or shape[0] != P:
                 raise ValueError(f"evict_rows: tensor {len(rows)} has shape {tuple(shape)}, {P} rows wanted")
-            if not t.is_contiguous():
-                t = t.contiguous()
+            if not t.is_contiguous() or t.is_conj() or (P == 1 and t.is_neg()):
+                t = _dense(t)
                 held.append(t)
             y = t.new_empty((keep, *shape[1:]))
             rows.append(y)
-            _ROW.pack_into(buf, at, t.data_ptr(), y.data_ptr(), 0, 0, t.nbytes // P if P else 0)
+            pack(buf, at, t.data_ptr(), y.data_ptr(), 0, 0, t.nbytes // P if P else 0)
             at += size
         for c, w in rms:
             k = c.numel()
@@ -291,7 +295,7 @@ def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=())
             held += (c, w)
             row = k // P if P else 0
             pairs.append((c.new_empty((keep, *c.shape[1:])), w.new_empty((keep * row + WINDOW - 1) // WINDOW)))
-            _ROW.pack_into(buf, at, c.data_ptr(), pairs[-1][0].data_ptr(), w.data_ptr(), pairs[-1][1].data_ptr(), row)
+            pack(buf, at, c.data_ptr(), pairs[-1][0].data_ptr(), w.data_ptr(), pairs[-1][1].data_ptr(), row)
             at += size
         ws_t, ws = _workspace(lib.gsr_evict_bytes(P), index)
         args = _lib.EvictArgs(P, 0 if weights is None else weights.shape[0], keep, recent, scores.data_ptr(),
@@ -414,14 +418,14 @@ class AdamW(torch.optim.Optimizer):
         packed = [_pack(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, origin if bits == 8 else None)
                   for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, origin) in calls.items()]
         if len(packed) > 1 or moved:
-            for call in packed:
-                call.check()
+            for args, origins, *_ in packed:
+                _lib.check(_lib.load().gsr_adamw_check(C.byref(args), _address(origins)))
         for st, betas, home in moved:
             # torch's corrections: 1 - beta ** t, of this step's betas
             for k in (0, 1):
                 torch.pow(betas[k], st["step"][2], out=st["step"][k])
         for call in packed:
-            call.launch()
+            _launch(call)
         for st, betas, home in moved:
             st["betas"] = betas
             if betas == home:

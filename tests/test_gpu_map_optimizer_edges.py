@@ -324,3 +324,33 @@ def test_a_refused_step_has_stepped_nothing(bits, what):
     opt.state[ps[1]] = good
     opt.step()
     assert [float(opt.state[p]["step"][2]) for p in ps] == [2.0] * 3
+
+
+# ---- layouts that torch has not resolved -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("P", [1, 3000])
+def test_lazy_conjugates_and_negatives(P):
+    """conj() and the imaginary part of a conjugate are marks on the same memory until something resolves them; one row of the latter is contiguous"""
+    gen = torch.Generator(device=DEV).manual_seed(57)
+    z = torch.randn(P, 2, generator=gen, device=DEV, dtype=torch.complex64)
+    neg = z.conj()[:, :1].imag
+    assert z.conj().is_conj() and z.conj().is_contiguous() and neg.is_neg()
+    s = torch.rand(P, generator=gen, device=DEV)
+    marked = torch.complex(s, -s).conj().imag
+    keep = (P + 2) // 3
+    kept, scores, rows, _ = MO().evict_rows(marked, keep, [z.conj(), neg, neg.t().contiguous().t()], weights=marked)
+    want, ws = O.evict(s.cpu().numpy(), keep, 0, s.cpu().numpy()[None])
+    assert np.array_equal(kept.cpu().numpy(), want) and np.array_equal(scores.cpu().numpy(), ws)
+    assert torch.equal(rows[0], z.conj().resolve_conj()[kept]) and torch.equal(rows[1], -z[:, :1].imag[kept]) and torch.equal(rows[2], rows[1])
+    out = []
+    for grad in (s, marked):
+        p, m, v = torch.ones(P, device=DEV), torch.zeros(P, device=DEV), torch.zeros(P, device=DEV)
+        MO().adamw_step([p], [grad], [m], [v], clocks(1, 0, (0.9, 0.999)), lr=0.1)
+        out.append((p, m, v, MO().grad_norm([grad], 1.0)))
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
+    if P == 1:
+        m, v, ck = torch.zeros(P, device=DEV), torch.zeros(P, device=DEV), clocks(1, 0, (0.9, 0.999))
+        with pytest.raises(ValueError, match="negative"):
+            MO().adamw_step([marked], [s], [m], [v], ck, lr=0.1)
+        assert float(ck[0][2]) == 0.0 and not bool(m.any())
