@@ -296,8 +296,9 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_adamw(OptArgs a)
 // Stored are u = sqrt(v) and r = m / u.
 //   u   the upper 13 bits of the float (sign, exponent, four bits of mantissa), minus 16 w + 1, in a byte; w, one byte per 256 elements,
 //       places the window: sixteen binades under the block's largest root.  0 stands for 0; what is positive but lies under the window is
-//       raised to code 1 (a smaller update, never a larger one).  Rounding is stochastic (19 random bits added under the kept ones: exactly
-//       unbiased inside a binade): with beta2 = 0.999 the moment moves by 0.1 % per step, and rounded to the nearest sixteenth it
+//       raised to code 1 (by a step, whose ratio is formed over the raised root, a smaller update, never a larger one; for an
+//       eviction see evict_bytes).  Rounding is stochastic (19 random bits added under the kept ones: each rounding
+//       exactly unbiased inside a binade): with beta2 = 0.999 the moment moves by 0.1 % per step, and rounded to the nearest sixteenth it
 //       would stand still wherever it once was.
 //   r   |m| <= B sqrt(v) whatever the gradients were, B = (1 - b1) / sqrt((1 - b2)(1 - b1^2 / b2)) (Cauchy-Schwarz over the two
 //       exponential sums; 7.27 for 0.9 / 0.999): 127 steps of B / 127 to either side, stochastic (13 bits).  A momentum quantised for
@@ -944,7 +945,8 @@ __device__ __forceinline__ void evict_chunk(const RowArgs& a, const RowTensor& t
 // has less than 4 GB (1.35 M rows of 180 bytes: 205 us, 240 with 64; as codes 240, 294).
 //
 // Codes of the 8-bit root change their block with their row: the float's upper bits move into the new block's window, exactly, but for
-// what lies under that window (raised to its lowest value, as by the step).
+// what lies under that window (raised to its lowest value).  The ratios are tensors of their own and copied as they are, so a raised
+// row's next update is what it would have been (m / sqrt(v) is the ratio either way), and the momentum that its bytes stand for grows with the root.
 template <bool CODES, class OFF>
 __device__ __forceinline__ void evict_bytes(const RowArgs& a, const RowTensor& t, long long base, uint32_t chunk)
 {

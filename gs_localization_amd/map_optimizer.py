@@ -254,7 +254,8 @@ def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=())
     score = decay * score + sum of weights.  The last `recent` rows stay whatever their score, and of the others the keep - recent with
     the largest (ties: the lower index; NaN counts as -inf).  tensors: [P, ...] each, of any types; rms: pairs (codes uint8 [P, ...], window)
     of 8-bit moments, re-coded for their new blocks -- exact, but for a root under its new window's sixteen binades, which
-    becomes that window's lowest value.
+    becomes that window's lowest value.  Its ratio (among `tensors`) is copied as it is: the row's next update stays what it was, the exp_avg
+    that the bytes stand for grows with the root, and gradients of the row's old size count for little until both have decayed.
     Returns (kept int64 [keep] ascending, scores [keep], [tensor [keep, ...]], [(codes, window)]); the inputs are not written."""
     lib = _lib.load()
     P, keep, recent = scores.numel(), int(keep), int(recent)

@@ -532,7 +532,8 @@ typedef struct gsr_moment_tensor { const uint8_t* rms; const int8_t* ratio; cons
 int gsr_adamw_moments(int n_tensors, const gsr_moment_tensor* tensors, double beta1, double beta2, int type, void* stream);
 
 /* One tensor that is compacted with the map: P rows of row_bytes bytes -> `keep` rows.  src_window (nullable): the tensor holds 8-bit
- * root codes with these windows; dst_window gets the (keep * row_bytes + 255) / 256 windows of the result. */
+ * root codes with these windows; dst_window gets the (keep * row_bytes + 255) / 256 windows of the result.  A root under its new window becomes that window's
+ * lowest value; the ratio that belongs to it is another tensor and copied as it is. */
 typedef struct gsr_row_tensor {
     const void* src; void* dst;
     const uint8_t* src_window; uint8_t* dst_window;

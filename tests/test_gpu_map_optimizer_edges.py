@@ -354,3 +354,38 @@ def test_lazy_conjugates_and_negatives(P):
         with pytest.raises(ValueError, match="negative"):
             MO().adamw_step([marked], [s], [m], [v], ck, lr=0.1)
         assert float(ck[0][2]) == 0.0 and not bool(m.any())
+
+
+# ---- codes that an eviction raises -------------------------------------------------------------------------------------------------------
+
+def test_step_after_an_eviction_that_raises_roots():
+    """Rows of roots 2^-30 of their new neighbours': a code becomes its new window's lowest, the ratio stays as it was.  What the bytes stand for is then
+    exp_avg = ratio x span / 127 x the raised root, and the next update is the one that the row would have got without the eviction
+    (its ratio's; never more than the span allows): here by a gradient of zero, to the roundings of two steps and eps."""
+    P = 1024
+    gen = torch.Generator(device=DEV).manual_seed(58)
+    small = torch.arange(P, device=DEV) < 256
+    p = torch.nn.Parameter(torch.zeros(P, 1, device=DEV))
+    opt = MO().AdamW([p], lr=0.1, eps=1e-30, state_bits=8, seed=2)
+    for _ in range(3):
+        p.grad = torch.randn(P, 1, generator=gen, device=DEV).abs() + 0.5
+        p.grad[small] *= 2.0 ** -30
+        opt.step()
+    whole = copy.deepcopy(opt)
+    (w,) = whole.param_groups[0]["params"]
+    kept, _, _ = opt.evict(torch.arange(P, device=DEV).float(), 824)
+    assert kept[0] == 200
+    (q,) = opt.param_groups[0]["params"]
+    raised = small[kept]
+    a, b = opt.state[q], whole.state[w]
+    assert torch.equal(a["ratio"], b["ratio"][kept]) and bool((a["rms"][raised] == 1).all())
+    (m,), (u,) = MO().moments_8bit([a["rms"]], [a["ratio"]], [a["window"]])
+    (m0,), (u0,) = MO().moments_8bit([b["rms"]], [b["ratio"]], [b["window"]])
+    assert bool((u[raised] > 1000 * u0[kept][raised]).all()) and torch.equal(u[~raised], u0[kept][~raised])
+    # the same ratio: m / u is the same in 32 bits but for two roundings each
+    assert float(((m / u) / (m0 / u0)[kept] - 1).abs().max()) <= 8 * E
+    q0, w0 = q.detach().clone(), w.detach().clone()
+    q.grad, w.grad = torch.zeros_like(q), torch.zeros_like(w)
+    opt.step(); whole.step()
+    x, y = n64(q.detach() - q0), n64(w.detach() - w0)[kept.cpu().numpy()]
+    assert (np.abs(x - y) <= 60 * E * np.abs(y) + 4 * E * np.abs(n64(q0))).all()
