@@ -389,3 +389,39 @@ def test_step_after_an_eviction_that_raises_roots():
     opt.step(); whole.step()
     x, y = n64(q.detach() - q0), n64(w.detach() - w0)[kept.cpu().numpy()]
     assert (np.abs(x - y) <= 60 * E * np.abs(y) + 4 * E * np.abs(n64(q0))).all()
+
+
+# ---- what the calls leave alone, and the types they give ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_grad_norm_writes_nothing(dtype, shift):
+    gen = torch.Generator(device=DEV).manual_seed(59)
+    gs = [Guarded((torch.randn(n, generator=gen, device=DEV) * 3).to(dtype), shift) for n in SIZES]
+    before = [g.t.clone() for g in gs]
+    for k in (1, len(gs)):
+        MO().grad_norm([g.t for g in gs[:k]], 1.0)
+    for g, b in zip(gs, before):
+        assert torch.equal(g.t, b)
+        g.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_moments_of_each_type(dtype, shift):
+    """The values that the codes stand for, computed in 32 bits (the unit's rounding and two products: 3 e) and rounded once: the roots' five bits are exact
+    in every type that has their exponents (float16: in windows 112 and 113, 2^-15 to 4, where its spacing is 2^-24 or finer than five bits)."""
+    gen = torch.Generator(device=DEV).manual_seed(60)
+    low, high = (112, 114) if dtype is torch.float16 else (60, 120)
+    ts = [random_codes(n, gen, shift, low, high) for n in SIZES]
+    before = [[x.t.clone() for x in q] for q in ts]
+    avg, root = MO().moments_8bit([q[0].t for q in ts], [q[1].t for q in ts], [q[2].t for q in ts], dtype=dtype)
+    for q, b, a, r in zip(ts, before, avg, root):
+        u = O.decode(q[0].t.cpu().numpy(), q[2].t.cpu().numpy())
+        m = n64(q[1].t) / 127 * O.span(0.9, 0.999) * u
+        assert a.dtype == r.dtype == dtype and a.shape == r.shape == q[0].t.shape
+        assert (n64(r) == u).all()
+        assert (np.abs(n64(a) - m) <= (3 * E + HALF[dtype] * (1 + 4 * E)) * np.abs(m) + (2.0 ** -25 if dtype is torch.float16 else 2.0 ** -149)).all()
+        for x, y in zip(q, b):
+            assert torch.equal(x.t, y)
+            x.check()
