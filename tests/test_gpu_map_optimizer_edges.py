@@ -425,3 +425,25 @@ def test_moments_of_each_type(dtype, shift):
         for x, y in zip(q, b):
             assert torch.equal(x.t, y)
             x.check()
+
+
+def test_spread_of_the_8_bit_root():
+    """What a byte for the root costs: after many steps of normal gradients it lies about the 32-bit moment's by a tenth.  A step moves a root by about 0.0005 x
+    0.968 of itself (E|g^2 - 1| = 0.968), which the rounding to steps of 1/32 to 1/16 of it turns into that times the step in variance; deviations
+    decay by 0.001 a step; so the variance settles between 0.968 x 0.0005 / 0.002 times 1/32 and 1/16: a deviation of 0.087 to 0.123, five standard
+    errors of 1 / sqrt(2 n) more.  It is unbiased, but its square is larger by the variance."""
+    n = 16384
+    gen = torch.Generator(device=DEV).manual_seed(61)
+    p, q, m, v = (torch.zeros(n, device=DEV) for _ in range(4))
+    rms, ratio, window = codes(n)
+    ca, cb = clocks(1, 0, (0.9, 0.999)), clocks(1, 0, (0.9, 0.999))
+    for _ in range(3000):
+        g = torch.randn(n, generator=gen, device=DEV) * 1e-4
+        MO().adamw_step([p], [g], [m], [v], ca, lr=0.0)
+        MO().adamw_step_8bit([q], [g], [rms], [ratio], [window], cb, lr=0.0, seed=6)
+    _, (u,) = MO().moments_8bit([rms], [ratio], [window])
+    r = u.double() / v.double().sqrt()
+    more = 5 / math.sqrt(2 * n)
+    assert 0.087 * (1 - more) < float(r.std()) < 0.123 * (1 + more)
+    assert abs(float(r.mean()) - 1) < 0.123 ** 2 / 2 + 5 * 0.123 / math.sqrt(n)          # (curvature of the root: under half the variance)
+    assert 0.087 ** 2 / 2 < float((r * r).mean()) - 1 < 0.123 ** 2 * 2
