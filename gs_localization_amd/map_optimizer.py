@@ -89,8 +89,10 @@ def _workspace(nbytes, index):
 
 
 def _dense(t):
-    """A dense tensor of t's values: strides, and what torch has only marked (a conjugate; the sign of its imaginary part, which is contiguous if it
-    is one element), are copied."""
+    """t, or a dense copy of its values: of strides, and of what torch has only marked (a conjugate; the sign of its imaginary part, which is
+    contiguous only as one element)."""
+    if t.is_contiguous() and not t.is_neg() and not t.is_conj():
+        return t
     return t.resolve_conj().resolve_neg().contiguous()
 
 
@@ -276,12 +278,12 @@ def evict_rows(scores, keep, tensors, recent=0, weights=None, decay=1.0, rms=())
     with _on(index) as stream:
         out = scores.new_empty(keep)
         kept = torch.empty(keep, dtype=torch.int64, device=scores.device)
-        at, pack = 0, _ROW.pack_into
+        at, pack, one = 0, _ROW.pack_into, P == 1
         for t in tensors:
             shape = t.shape
             if not shape or shape[0] != P:
                 raise ValueError(f"evict_rows: tensor {len(rows)} has shape {tuple(shape)}, {P} rows wanted")
-            if not t.is_contiguous() or t.is_conj() or (P == 1 and t.is_neg()):
+            if t.is_conj() or one or not t.is_contiguous():
                 t = _dense(t)
                 held.append(t)
             y = t.new_empty((keep, *shape[1:]))
