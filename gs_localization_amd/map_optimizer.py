@@ -390,36 +390,43 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         calls, grads, moved, place = {}, [], [], -1
         for group in self.param_groups:
-            betas = tuple(group["betas"])
+            betas, bits, lr, decay = tuple(group["betas"]), group["state_bits"], group["lr"], group["weight_decay"]
             home = group.setdefault("state_betas", betas)
+            call = calls.setdefault((bits, betas, group["eps"]), [])
             for p in group["params"]:
                 place += 1          # (of a parameter, whichever others are stepped and in how many calls: its random bits are its own)
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                if p.grad.layout is not torch.strided:
+                if g.layout is not torch.strided:
                     raise RuntimeError("AdamW does not support sparse gradients")
-                _device((p,), "AdamW")
                 st = self.state[p] if p in self.state else None
                 if not st:
-                    st = self._init_state(p, group["state_bits"])
+                    _device((p,), "AdamW")
+                    st = self._init_state(p, bits)
                     if betas != home:
                         st["betas"] = betas
                 was = st.get("betas", home)
                 if was != betas:
-                    if group["state_bits"] == 8 and torch.cuda.is_current_stream_capturing():
+                    if bits == 8 and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("AdamW: the first 8-bit step with other betas cannot be captured (every replay would read the ratios with the old ones): step once before")
                     moved.append((st, betas, home))
-                call = calls.setdefault((group["state_bits"], betas, group["eps"]), ([], [], [], [], [], [], [], [], []))
-                for x, y in zip(call, (p, p.grad, *((st["exp_avg"], st["exp_avg_sq"], None) if group["state_bits"] == 32 else
-                                                    (st["rms"], st["ratio"], st["window"])), st["step"], group["lr"], group["weight_decay"], (was, place))):
-                    x.append(y)
-                grads.append(p.grad)
+                call.append((p, g, st["exp_avg"], st["exp_avg_sq"], st["step"], lr, decay) if bits == 32 else
+                            (p, g, st["rms"], st["ratio"], st["step"], lr, decay, st["window"], (was, place)))
+                grads.append(g)
         if not grads:
             return loss
         clip = None if self.max_norm is None else grad_norm(grads, self.max_norm)
         # (made whole or not at all: everything is checked before anything is launched)
-        packed = [_pack(bits, "AdamW", p, g, a, b, w if bits == 8 else None, clock, lr, betas, eps, wd, clip, self.seed, origin if bits == 8 else None)
-                  for (bits, betas, eps), (p, g, a, b, w, clock, lr, wd, origin) in calls.items()]
+        packed = []
+        for (bits, betas, eps), call in calls.items():
+            if not call:
+                continue
+            p, g, a, b, clock, lr, decay, *coded = zip(*call)
+            window, origin = coded or (None, None)
+            if coded and not moved and origin[-1][1] == len(p) - 1:
+                origin = None          # (this step's betas, places in the list)
+            packed.append(_pack(bits, "AdamW", p, g, a, b, window, clock, lr, betas, eps, decay, clip, self.seed, origin))
         if len(packed) > 1 or moved:
             for args, origins, *_ in packed:
                 _lib.check(_lib.load().gsr_adamw_check(C.byref(args), _address(origins)))

@@ -1,7 +1,7 @@
 """BASELINE.json config 4 and nothing else: N train.py-style steps (tests/train_replay.py: package (A) forward at 1296x840, SH1,
 white background, random camera per step; fused loss epilogue; backward; densification statistics; torch Adam) at a fixed number
 of Gaussians -- the command the rocprofv3 passes of tools/profile_r04.sh run.  argv: steps [P] [optimiser: torch (default), 32 or 8 =
-gs_localization_amd.map_optimizer.AdamW with moments of that many bits]."""
+gs_localization_amd.map_optimizer.AdamW with moments of that many bits].  Prints the time of a step and the mean losses of the steps' fifths."""
 import sys, os, time
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch
@@ -17,7 +17,8 @@ if opt != "torch":
 for it in range(1, 4):
     tr.step(it)
 torch.cuda.synchronize(); t0 = time.perf_counter()
-for it in range(4, 4 + steps):
-    tr.step(it)
+losses = [tr.step(it) for it in range(4, 4 + steps)]
 torch.cuda.synchronize()
-print("train steps", steps, "P", P, "optimiser", opt, "ms/step %.3f" % (1e3 * (time.perf_counter() - t0) / steps))
+ms = 1e3 * (time.perf_counter() - t0) / steps
+losses = torch.stack([x.detach().reshape(()) for x in losses]).double().cpu()
+print("train steps", steps, "P", P, "optimiser", opt, "ms/step %.3f" % ms, "mean losses", " ".join("%.5f" % float(x.mean()) for x in losses.chunk(5)))
