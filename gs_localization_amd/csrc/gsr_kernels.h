@@ -1934,7 +1934,7 @@ __device__ __forceinline__ uint32_t seg_load_u(const uint32_t* p) { return __hip
 
 // Record layout: what the walk reads per list entry is a (16 B), the first half of b (8 B) and c (16 B), and the fields sit
 // next to each other as operand PAIRS: (x, y) - (px, py), (B2, C2) * dy, (r, g) * w, (b, depth) * w.  (The build switches the packed fp32 instructions
-// off: two plain operations each, same bits and, measured, the same rate.)
+// off: two plain operations each, the same bits; pose loop +0.7 % on S-1M-640, -0.9 % on S-3M-cam.)
 typedef float gsr_f32x2 __attribute__((ext_vector_type(2)));
 typedef float gsr_f32x4 __attribute__((ext_vector_type(4)));
 struct SplatLDS {

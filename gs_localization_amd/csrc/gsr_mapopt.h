@@ -1,4 +1,4 @@
-// gsr_mapopt.h -- the optimiser step of a Gaussian map and the pruning that goes with it: what gaussian_splatting/train.py:149-157 leaves
+// gsr_mapopt.h -- the optimiser step of a Gaussian map and the pruning that goes with it: what gaussian_splatting/train.py:155-157 leaves
 // to torch (Adam over six tensors, ~12 launches each; the rewriting of its state at every prune, scene/gaussian_model.py:269-300).
 //
 //   k_grad_norm, k_grad_norm_finish   the 2-norm over many tensors and the coefficient that clips it, on the device
@@ -44,8 +44,7 @@ typedef uint32_t opt_u2 __attribute__((ext_vector_type(2)));
 typedef __bf16 opt_b4 __attribute__((ext_vector_type(4)));
 typedef _Float16 opt_h4 __attribute__((ext_vector_type(4)));
 // STREAM: past the caches (non-temporal), for a launch whose data do not fit the 256 MB behind the L2 anyway: without it the lines
-// that a step leaves there only push out one another.  AdamW over 34.5 M elements (966 MB): 168 us with, 189 without; over 4.6 M (129 MB)
-// 28.6 with, 24.5 without -- the rule is opt_stream() (gsr_mapopt_api.h).
+// that a step leaves there only push out one another.  The rule is opt_stream() (gsr_mapopt_api.h), with both sides measured.
 template <bool STREAM, class T> __device__ __forceinline__ T opt_get(const T* p) { return STREAM ? __builtin_nontemporal_load(p) : *p; }
 template <bool STREAM, class T> __device__ __forceinline__ void opt_put(T* p, T x) { if (STREAM) __builtin_nontemporal_store(x, p); else *p = x; }
 template <int TYPE, bool STREAM>
@@ -189,8 +188,10 @@ __device__ __forceinline__ float opt_uniform(float x) { return __uint_as_float(_
 // launch of up to GSR_OPT_TICKETS workgroups does it by itself: a workgroup draws a ticket when it is done (the fourth word of the
 // launch's first clock, zero between launches), and the one that drew the last advances the clocks.  No fence: nothing but "has read" is
 // handed over, and what a wave has stored it has computed from the clock (a release at device scope writes the XCD's L2 back, 57 ns
-// per workgroup).  Same-address atomics take turns, 5 ns each, so a larger launch leaves it to k_adamw_advance behind it: 34.5 M
-// elements, 8424 workgroups: 302 us with tickets and fences, 209 with tickets, 167 + 4 with the launch.
+// per workgroup).  Same-address atomics take turns, so a larger launch leaves it to k_adamw_advance behind it: 34.5 M
+// elements, 8424 workgroups: 302 us with tickets and fences, 209 with tickets, 167 + 4 with the launch.  A tensor stepped again and again, with
+// tickets / with the launch: 256 workgroups 9.4 / 11.1 us, 384 11.4 / 11.1, 512 13.5 / 11.3, 768 37 / 16, 1024 62 / 20 (8 bits 10.2 / 11.4,
+// 12.0 / 11.5, 13.9 / 11.5, 17.8 / 13.7, 21.6 / 17.7): 512 is not far above the border.
 #define GSR_OPT_TICKETS 512
 struct OptRates { float shrink, rate, unbias; uint32_t key; };
 __device__ __forceinline__ OptRates opt_rates(const OptArgs& a, const OptTensor& t)
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(GSR_OPT_THREADS) k_moments8(MomentArgs a)
 #define GSR_EV_COPIES 8         // of the first histogram in LDS: its bins are exponents, a wave's lanes meet in few of them
 #define GSR_EV_TILE 1024        // rows of a tile, or a multiple of it
 #define GSR_EV_TILES 2048       // tiles at most: every workgroup adds up its predecessors' counts by itself
-#define GSR_EV_SMALL 8192       // rows up to which one workgroup does it all
+#define GSR_EV_SMALL 8192       // rows up to which one workgroup does it all (a call at 8192 rows: 21 us for the six launches' 29; with 16 views 27 for 29)
 
 struct EvictArgs {
     int P, views, old, k;       // old = P - recent: the rows that compete; k of them stay

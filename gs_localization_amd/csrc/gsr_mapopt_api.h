@@ -9,7 +9,9 @@ static_assert(sizeof(gsr::OptArgs) <= 4096 && sizeof(gsr::RowArgs) <= 4096 && si
 // bytes for an element, so the card's 288 GB hold no more.
 const long long kOptMaxElements = 1LL << 35;
 const int kOptGrid = 2048;                            // workgroups of the norm's launches: eight per CU, each walks chunks
-// Past the caches from 256 MB on (what lies behind the L2): see opt_get.
+// Past the caches (opt_get) from 256 MB on, what lies behind the L2; `bytes` counts what a step reads.  32-bit moments, cached / past the caches, a step
+// that follows its like: 128 MB 38 / 43 us, 256 71 / 81, 320 95 / 103, 384 135 / 122, 640 222 / 199; behind a GB of other work, as in a
+// training step: 62 / 48, 105 / 84, 128 / 106, 146 / 125, 231 / 201 (8 bits alike: 40 / 42, 72 / 78, 91 / 95, 119 / 112, 204 / 180).
 bool opt_stream(long long bytes) { return bytes > 256LL << 20; }
 bool opt_type_ok(int t) { return t == GSR_TYPE_F32 || t == GSR_TYPE_BF16 || t == GSR_TYPE_F16; }
 long long opt_size(int t) { return t == GSR_TYPE_F32 ? 4 : 2; }
@@ -262,7 +264,7 @@ int evict_rows(const gsr_evict_args* a)
     e.P = a->P; e.views = a->n_views; e.old = a->P - a->recent; e.k = a->keep - a->recent; e.decay = a->decay;
     e.scores = a->scores; e.weights = a->weights; e.total = w.total; e.hist = w.hist; e.found = w.found; e.counts = w.counts;
     e.kept = a->kept; e.scores_out = a->scores_out;
-    if (a->P <= GSR_EV_SMALL) {          // one workgroup, one launch: at 2000 rows 15 us for the six's 25
+    if (a->P <= GSR_EV_SMALL) {          // one workgroup, one launch
         hipLaunchKernelGGL(k_evict_small, dim3(1), dim3(1024), 0, st, e);
         LAUNCHCHK("k_evict_small");
     } else {

@@ -1,7 +1,7 @@
 """The optimiser step of a Gaussian map and the pruning that goes with it, on hand-written HIP kernels (include/gsr.h: gsr_grad_norm,
 gsr_adamw_step, gsr_adamw_moments, gsr_evict_rows).
 
-gaussian_splatting/train.py:156-158 steps torch.optim.Adam over the six tensors of a map and gaussian_splatting/scene/
+gaussian_splatting/train.py:155-157 steps torch.optim.Adam over the six tensors of a map and gaussian_splatting/scene/
 gaussian_model.py:269-328 rewrites its state whenever splats are pruned or added.  Here
 
   AdamW           an optimiser with torch's constructor, groups and state ("exp_avg", "exp_avg_sq"): one launch for all tensors; moments
@@ -10,9 +10,9 @@ gaussian_model.py:269-328 rewrites its state whenever splats are pruned or added
   grad_norm, adamw_step, adamw_step_8bit, moments_8bit, evict_rows      the operators by themselves
   compositing_weights                                                   what evict_rows accumulates, from the rasterizer
 
-No entry point reads anything back, and each runs on its tensors' device and that device's current stream; two steps of the same tensors
-must not overlap, as with any operation in place.  Nothing falls back to torch
-or to the CPU: tensors elsewhere are refused.  Tensors that a step writes must be contiguous and must not overlap (refused); the
+No operator reads anything back, and each runs on its tensors' device and that device's current stream; two steps of the same tensors
+must not overlap, as with any operation in place.  (compositing_weights is a forward and a backward of the rasterizer, which may read back and is not made
+for capture.)  Nothing falls back to torch or to the CPU: tensors elsewhere are refused.  Tensors that a step writes must be contiguous and must not overlap (refused); the
 step counts live on the device, so a captured graph counts on when it is replayed."""
 import ctypes as C
 import math
@@ -213,6 +213,7 @@ def adamw_step_8bit(params, grads, rms, ratio, window, clocks, lr, betas=(0.9, 0
     in 127 steps of the largest it can be), window (uint8, one per 256 elements of the flattened tensor: which sixteen binades rms
     covers); all zero before the first step.  Rounding is stochastic, from `seed`, the step, the tensor's place in the list and the element's: the same
     call on the same state gives the same bits.  Needs beta1^2 < beta2.  moments_8bit reads them.
+    With beta2 = 0.999 the stored root walks about the 32-bit moment's with a standard deviation of a tenth, and so does each element's rate.
     The largest that the ratio can be depends on the betas.  state_betas: those of the last step that stored the ratios, one pair or one per
     tensor, where they are not this step's; ratios are read with them and stored with `betas`."""
     if state_betas is not None:

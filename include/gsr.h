@@ -476,7 +476,7 @@ int gsr_training_loss(int width, int height, const float* image, const float* gt
 int gsr_densification_stats(int P, const int* radii, const float* dL_dmean2D, float* max_radii2D,
                             float* xyz_gradient_accum, float* denom, void* stream);
 
-/* The optimiser step of a map (what gaussian_splatting/train.py:156-158 leaves to torch.optim.Adam: six tensors, a dozen launches
+/* The optimiser step of a map (what gaussian_splatting/train.py:155-157 leaves to torch.optim.Adam: six tensors, a dozen launches
  * each) and the pruning that goes with it (prune_points / _prune_optimizer, scene/gaussian_model.py:269-300).  Elements are dense;
  * any number of tensors, of any sizes (zero included), in one call: 40 per launch.  No entry point here waits, reads anything back or
  * uses memory beyond its arguments, so all of them can be captured into a graph; the step count lives on the device. */
